@@ -54,6 +54,7 @@ typedef enum {
   B2R_I64 = 4,
   B2R_I16 = 5,
   B2R_U32 = 6,
+  B2R_BF16 = 7, /* the vocabulary operators only (b2r_embedding_*, b2r_topk_distill*, b2r_sample_tokens) */
   /* {int32 key; V value} pairs, laid out like raft::KeyValuePair<int, V> (core/kvp.hpp:20-27) */
   B2R_KVP_I32_F32 = 16,
   B2R_KVP_I32_F64 = 17,
@@ -247,6 +248,59 @@ B2R_API int b2r_matrix_argmax(void* out,
                               int64_t n_rows,
                               int64_t n_cols,
                               b2r_stream_t stream);
+
+/*
+ * Vocabulary operators: the two ends of a language model, where rows are named by token or run over the whole
+ * vocabulary. No counterpart in the reference; they are the gather, the keyed row sum, the log-sum-exp row
+ * reduction and the row selection next to the reductions above. Common to all of them: data types B2R_F32,
+ * B2R_F16 and B2R_BF16, arithmetic in 32 bits or more, one rounding at the end; row-major matrices with a row
+ * stride (ld, in elements, at least the number of columns) and any element alignment; tokens B2R_I32 or B2R_I64.
+ * Sizes are at most 2^31 - 1 (B2R_ERR_TOO_LARGE above), offsets are 64-bit.
+ *
+ * b2r_embedding_lookup:  out[i][0..n_cols) = scale * table[tokens[i]][0..n_cols). A token outside [0, vocab) is no
+ * token (padding): its row of `out` is zero and nothing is read for it. out and table have the same type and must
+ * not overlap.
+ */
+B2R_API int b2r_embedding_lookup(void* out,
+                                 int64_t ldo,
+                                 const void* table,
+                                 int64_t ldt,
+                                 const void* tokens,
+                                 int32_t dtype,
+                                 int32_t token_dtype,
+                                 int64_t n_tokens,
+                                 int64_t n_cols,
+                                 int64_t vocab,
+                                 double scale,
+                                 b2r_stream_t stream);
+
+/*
+ * Gradient of b2r_embedding_lookup with respect to the table:
+ *     grad_table[v][0..n_cols) (+)= scale * sum over i with tokens[i] == v of grad_out[i][0..n_cols)
+ * accumulate == 0: every row of grad_table [vocab x n_cols] is written, with zeros where no token names it;
+ * otherwise the sums are added to what the rows hold and rows that no token names are left alone. Tokens outside
+ * [0, vocab) add nothing. Sums are fp32, rounded once; their order depends on the positions alone, so results
+ * repeat bit for bit. grad_out of type `dtype`, grad_table of the same type or B2R_F32; they must not overlap.
+ * `workspace`: b2r_embedding_grad_workspace_bytes() bytes (256-byte aligned), or NULL.
+ */
+B2R_API int b2r_embedding_grad(void* grad_table,
+                               int64_t ldg,
+                               int32_t table_dtype,
+                               const void* grad_out,
+                               int64_t ldo,
+                               int32_t dtype,
+                               const void* tokens,
+                               int32_t token_dtype,
+                               int64_t n_tokens,
+                               int64_t n_cols,
+                               int64_t vocab,
+                               double scale,
+                               int32_t accumulate,
+                               void* workspace,
+                               size_t workspace_bytes,
+                               b2r_stream_t stream);
+
+B2R_API size_t b2r_embedding_grad_workspace_bytes(int64_t n_tokens, int64_t n_cols, int64_t vocab);
 
 /*
  * Column sums of a row-major fp32 matrix without any allocation:

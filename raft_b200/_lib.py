@@ -12,7 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libraft_b200.so")
 # b2r_status
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_TOO_LARGE, ERR_TIMEOUT = 0, 1, 2, 3, 4, 5
 # b2r_dtype
-F32, F64, F16, I32, I64, I16, U32 = 0, 1, 2, 3, 4, 5, 6
+F32, F64, F16, I32, I64, I16, U32, BF16 = 0, 1, 2, 3, 4, 5, 6, 7
 KVP_I32_F32, KVP_I32_F64, KVP_I32_I16, KVP_I32_I32 = 16, 17, 18, 19
 # b2r_layout / b2r_apply
 ROW_MAJOR, COL_MAJOR = 0, 1
@@ -61,6 +61,10 @@ SIGNATURES = {
     "b2r_row_normalize": (ctypes.c_int, [_vp, _vp, _i32, _i64, _i64, _i32, _dbl, _vp]),
     "b2r_matrix_argmin": (ctypes.c_int, [_vp, _i32, _vp, _i32, _i64, _i64, _vp]),
     "b2r_matrix_argmax": (ctypes.c_int, [_vp, _i32, _vp, _i32, _i64, _i64, _vp]),
+    "b2r_embedding_lookup": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i32, _i32, _i64, _i64, _i64, _dbl, _vp]),
+    "b2r_embedding_grad": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i64, _i64, _i64, _dbl, _i32,
+                                          _vp, _sz, _vp]),
+    "b2r_embedding_grad_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "b2r_column_sum_f32_noalloc": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _dbl, _vp]),
     "b2r_column_sum_f32_noalloc_max_scratch": (_sz, []),
     "b2r_apply_final": (ctypes.c_int, [_vp, _i32, _i64, _i32, _dbl, _vp]),

@@ -12,6 +12,9 @@ the reference:
   reduce_rows_by_key   linalg/reduce_rows_by_key.cuh:140-181
   reduce_cols_by_key   linalg/reduce_cols_by_key.cuh:76-102
 
+Beside them, without a counterpart in the reference, the vocabulary operators: embedding_lookup, embedding_grad,
+topk_distill, topk_distill_grad, topk_distill_step and sample_tokens.
+
 Shape errors raise ValueError where the reference's RAFT_EXPECTS raises raft::logic_error;
 unsupported type / operator combinations raise B2RError (raft::exception in the reference).
 Functors are named by strings because a C ABI cannot carry a device lambda; the C++ headers
@@ -315,6 +318,156 @@ def reduce_cols_by_key_workspace_bytes(data, nkeys):
     with _on(data.device):
         return L.load().b2r_reduce_cols_by_key_workspace_bytes(data.data_ptr(), _DTYPES[data.dtype], nrows, ncols,
                                                                nkeys)
+
+
+_VOCAB_DTYPES = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
+_TOKEN_DTYPES = {torch.int32: L.I32, torch.int64: L.I64}
+
+
+def _on_device_of(t, name, other):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.device != other.device:
+        raise ValueError(f"{name} must be on {other.device}")
+
+
+def _row_stride(t, name):
+    """Row stride of a row-major matrix (rows may be further apart than they are long)."""
+    n_rows, n_cols = t.shape
+    s0, s1 = t.stride()
+    if n_cols > 1 and s1 != 1:
+        raise ValueError(f"{name} must be row-major")
+    if n_rows <= 1:
+        return n_cols
+    if s0 < n_cols:
+        raise ValueError(f"{name} must be row-major")
+    return s0
+
+
+def _overlap(a, b):
+    """Whether the memory that two tensors span overlaps."""
+    def span(t):
+        if t.numel() == 0:
+            return 0, 0
+        lo = t.data_ptr()
+        return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _workspace(workspace, like):
+    if workspace is None:
+        return None, 0
+    _on_device_of(workspace, "workspace", like)
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def embedding_lookup(table, tokens, scale=1.0, out=None):
+    """out[i, :] = scale * table[tokens[i], :], the rows of an embedding table by token.
+
+    table: [vocab x n_cols] row-major (rows may be strided), float32 / float16 / bfloat16; tokens: int32 / int64 of
+    any shape, contiguous; out: [tokens.numel() x n_cols] of the table's type (default: a new tensor of shape
+    tokens.shape + (n_cols,)). A token outside [0, vocab) - the -1 of padded positions - gives a row of zeros.
+    Returns out."""
+    _require_cuda(table, "table")
+    if table.dim() != 2:
+        raise ValueError("table must be a matrix")
+    _on_device_of(tokens, "tokens", table)
+    dt, tt = _VOCAB_DTYPES.get(table.dtype), _TOKEN_DTYPES.get(tokens.dtype)
+    if dt is None or tt is None:
+        raise L.B2RError(L.ERR_UNSUPPORTED, "embedding_lookup")
+    if not tokens.is_contiguous():
+        raise ValueError("tokens must be contiguous")
+    vocab, n_cols = table.shape
+    n = tokens.numel()
+    ldt = _row_stride(table, "table")
+    if out is None:
+        out = torch.empty(tokens.shape + (n_cols,), dtype=table.dtype, device=table.device)
+        ldo = n_cols
+    else:
+        _on_device_of(out, "out", table)
+        if out.dtype != table.dtype:
+            raise ValueError("out and table must have the same element type")
+        rows = _as_rows(out, n, n_cols, "out")
+        ldo = _row_stride(rows, "out")
+        if _overlap(out, table) or _overlap(out, tokens):
+            raise ValueError("out must not overlap table or tokens")
+    with _on(table.device):
+        st = L.load().b2r_embedding_lookup(out.data_ptr(), ldo, table.data_ptr(), ldt, tokens.data_ptr(), dt, tt, n,
+                                           n_cols, vocab, float(scale), _stream_ptr(table.device))
+    L.check(st, "b2r_embedding_lookup")
+    return out
+
+
+def _as_rows(t, n, n_cols, name):
+    """`t` as a matrix of n rows of n_cols, without a copy."""
+    if t.dim() < 1 or t.shape[-1] != n_cols or t.numel() != n * n_cols:
+        raise ValueError(f"{name} must have {n} rows of {n_cols}")
+    if t.dim() == 2:
+        return t
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous or a row-major matrix")
+    return t.reshape(n, n_cols)
+
+
+def embedding_grad(grad_out, tokens, vocab, scale=1.0, grad_table=None, accumulate=False, out_dtype=None,
+                   workspace=None):
+    """Gradient of embedding_lookup with respect to its table:
+    grad_table[v, :] = scale * sum of grad_out[i, :] over the positions i with tokens[i] == v.
+
+    grad_out: [tokens.numel() x n_cols] (or tokens.shape + (n_cols,), contiguous), float32 / float16 / bfloat16;
+    grad_table: [vocab x n_cols] of the same type or float32 (default: a new tensor of type `out_dtype`, else
+    grad_out's). With `accumulate` the sums are added to what grad_table holds; without, rows that no token names
+    are set to zero. Tokens outside [0, vocab) add nothing. Sums are in float32 in an order that the positions alone
+    determine: results repeat bit for bit. `workspace` (uint8, see embedding_grad_workspace_bytes) keeps the call
+    allocation-free. Returns grad_table."""
+    _require_cuda(grad_out, "grad_out")
+    _on_device_of(tokens, "tokens", grad_out)
+    dt, tt = _VOCAB_DTYPES.get(grad_out.dtype), _TOKEN_DTYPES.get(tokens.dtype)
+    if dt is None or tt is None:
+        raise L.B2RError(L.ERR_UNSUPPORTED, "embedding_grad")
+    if not tokens.is_contiguous():
+        raise ValueError("tokens must be contiguous")
+    if grad_out.dim() < 1:
+        raise ValueError("grad_out must be a matrix")
+    vocab, n, n_cols = int(vocab), tokens.numel(), grad_out.shape[-1]
+    if vocab < 0:
+        raise ValueError("vocab must not be negative")
+    ldo = _row_stride(_as_rows(grad_out, n, n_cols, "grad_out"), "grad_out")
+    if grad_table is None:
+        if accumulate:
+            raise ValueError("accumulate needs a grad_table")
+        grad_table = torch.empty((vocab, n_cols), dtype=out_dtype or grad_out.dtype, device=grad_out.device)
+        ldg = n_cols
+    else:
+        _on_device_of(grad_table, "grad_table", grad_out)
+        if tuple(grad_table.shape) != (vocab, n_cols):
+            raise ValueError("grad_table is not of size vocab * n_cols")
+        if out_dtype is not None and out_dtype != grad_table.dtype:
+            raise ValueError("grad_table is not of type out_dtype")
+        ldg = _row_stride(grad_table, "grad_table")
+        if _overlap(grad_table, grad_out) or _overlap(grad_table, tokens):
+            raise ValueError("grad_table must not overlap grad_out or tokens")
+    if grad_table.dtype not in (grad_out.dtype, torch.float32):
+        raise L.B2RError(L.ERR_UNSUPPORTED, "embedding_grad")
+    ws_ptr, ws_bytes = _workspace(workspace, grad_out)
+    with _on(grad_out.device):
+        st = L.load().b2r_embedding_grad(
+            grad_table.data_ptr(), ldg, _VOCAB_DTYPES[grad_table.dtype], grad_out.data_ptr(), ldo, dt,
+            tokens.data_ptr(), tt, n, n_cols, vocab, float(scale), 1 if accumulate else 0, ws_ptr, ws_bytes,
+            _stream_ptr(grad_out.device))
+    L.check(st, "b2r_embedding_grad")
+    return grad_table
+
+
+def embedding_grad_workspace_bytes(grad_out, vocab):
+    """Bytes of workspace that embedding_grad takes for rows of grad_out's shape."""
+    n_cols = grad_out.shape[-1]
+    n = grad_out.numel() // n_cols if n_cols else 0
+    with _on(grad_out.device):
+        return L.load().b2r_embedding_grad_workspace_bytes(n, n_cols, int(vocab))
 
 
 def last_kernel_status(device, clear=True):
