@@ -303,6 +303,61 @@ B2R_API int b2r_embedding_grad(void* grad_table,
 B2R_API size_t b2r_embedding_grad_workspace_bytes(int64_t n_tokens, int64_t n_cols, int64_t vocab);
 
 /*
+ * Distillation from a teacher's top logits. Row r of `logits` [n_rows x vocab] are a student's logits z, row r of
+ * ids / teacher [n_rows x k] the teacher's list: tokens and their logits y. With T = temperature,
+ *     p = softmax(y / T) over the entries whose token lies in [0, vocab),   q = softmax(z / T) over the vocabulary
+ *     loss[r] = T^2 * sum_k p_k (log p_k - log q[ids_k])                    lse[r] = log sum_v exp(z_v / T)
+ *     grad[r][v] = grad_loss[r] * T * (q_v - sum of p_k with ids_k == v)    (= grad_loss[r] * d loss[r] / d z_v)
+ * A token named twice counts twice. A row without any valid entry, or whose valid entries are all -inf, has loss 0
+ * and gradient 0 whatever its logits hold; elsewhere NaN and +inf logits give NaN.
+ *  b2r_topk_distill       loss and lse (either may be NULL), and with `grad` non-NULL the gradient in the same pass
+ *                         over the logits: one read and one write of the matrix.
+ *  b2r_topk_distill_grad  the gradient alone, from the lse of an earlier call.
+ * logits and grad have type `dtype`; teacher is B2R_F32, B2R_F16 or B2R_BF16; loss, lse, grad_loss are fp32.
+ * k is at most 1024 (B2R_ERR_TOO_LARGE), temperature between 1e-30 and 1e30. `grad` may be `logits` (same pointer and stride), else it must not
+ * overlap them. The gradient is written fastest when both matrices start on the same 16-byte phase and have the
+ * same stride modulo 16 bytes.
+ */
+B2R_API int b2r_topk_distill(float* loss,
+                             float* lse,
+                             void* grad,
+                             int64_t ldg,
+                             const float* grad_loss,
+                             const void* logits,
+                             int64_t ldl,
+                             int32_t dtype,
+                             const void* ids,
+                             int64_t ldi,
+                             int32_t id_dtype,
+                             const void* teacher,
+                             int64_t ldt,
+                             int32_t teacher_dtype,
+                             int64_t n_rows,
+                             int64_t vocab,
+                             int64_t k,
+                             double temperature,
+                             b2r_stream_t stream);
+
+B2R_API int b2r_topk_distill_grad(void* grad,
+                                  int64_t ldg,
+                                  const float* lse,
+                                  const float* grad_loss,
+                                  const void* logits,
+                                  int64_t ldl,
+                                  int32_t dtype,
+                                  const void* ids,
+                                  int64_t ldi,
+                                  int32_t id_dtype,
+                                  const void* teacher,
+                                  int64_t ldt,
+                                  int32_t teacher_dtype,
+                                  int64_t n_rows,
+                                  int64_t vocab,
+                                  int64_t k,
+                                  double temperature,
+                                  b2r_stream_t stream);
+
+/*
  * Column sums of a row-major fp32 matrix without any allocation:
  *     out[j] = final_op(sum over i of in[i][j]),   in [n_rows x n_cols], out [n_cols]
  * This entry point has no counterpart in the reference. It is b2r_reduce's column path

@@ -65,6 +65,10 @@ SIGNATURES = {
     "b2r_embedding_grad": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _i32, _i64, _i64, _i64, _dbl, _i32,
                                           _vp, _sz, _vp]),
     "b2r_embedding_grad_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "b2r_topk_distill": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _i32,
+                                        _i64, _i64, _i64, _dbl, _vp]),
+    "b2r_topk_distill_grad": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _i32,
+                                             _i64, _i64, _i64, _dbl, _vp]),
     "b2r_column_sum_f32_noalloc": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _dbl, _vp]),
     "b2r_column_sum_f32_noalloc_max_scratch": (_sz, []),
     "b2r_apply_final": (ctypes.c_int, [_vp, _i32, _i64, _i32, _dbl, _vp]),

@@ -470,6 +470,109 @@ def embedding_grad_workspace_bytes(grad_out, vocab):
         return L.load().b2r_embedding_grad_workspace_bytes(n, n_cols, int(vocab))
 
 
+def _distill_args(logits, teacher_ids, teacher_logits, temperature, where):
+    """The checks the distillation calls share: (dtype, id dtype, teacher dtype, row strides, rows, vocab, k)."""
+    _require_cuda(logits, "logits")
+    _on_device_of(teacher_ids, "teacher_ids", logits)
+    _on_device_of(teacher_logits, "teacher_logits", logits)
+    if logits.dim() != 2 or teacher_ids.dim() != 2 or teacher_logits.dim() != 2:
+        raise ValueError("logits, teacher_ids and teacher_logits must be matrices")
+    dt, it, tt = (_VOCAB_DTYPES.get(logits.dtype), _TOKEN_DTYPES.get(teacher_ids.dtype),
+                  _VOCAB_DTYPES.get(teacher_logits.dtype))
+    if dt is None or it is None or tt is None:
+        raise L.B2RError(L.ERR_UNSUPPORTED, where)
+    n, vocab = logits.shape
+    if teacher_ids.shape[0] != n or teacher_ids.shape != teacher_logits.shape:
+        raise ValueError("teacher_ids and teacher_logits must have a row of the same length for every row of logits")
+    if not 1e-30 <= float(temperature) <= 1e30:
+        raise ValueError("temperature must be positive and finite (1e-30 to 1e30)")
+    return (dt, it, tt, _row_stride(logits, "logits"), _row_stride(teacher_ids, "teacher_ids"),
+            _row_stride(teacher_logits, "teacher_logits"), n, vocab, teacher_ids.shape[1])
+
+
+def _per_row(t, name, n, logits):
+    """A contiguous float32 vector with an element per row of logits."""
+    _on_device_of(t, name, logits)
+    if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous float32 of size n_rows")
+    return t
+
+
+def _grad_like(grad, logits, ldl):
+    """`grad`, checked, or a new matrix with logits' row stride (so that rows of both have the same alignment)."""
+    if grad is None:
+        n, vocab = logits.shape
+        grad = torch.empty_strided((n, vocab), (max(ldl, 1), 1), dtype=logits.dtype, device=logits.device)
+        return grad, ldl
+    _on_device_of(grad, "grad", logits)
+    if grad.dtype != logits.dtype or grad.shape != logits.shape:
+        raise ValueError("grad must have the shape and element type of logits")
+    ldg = _row_stride(grad, "grad")
+    if _overlap(grad, logits) and (grad.data_ptr() != logits.data_ptr() or ldg != ldl):
+        raise ValueError("grad must be logits or not overlap them")
+    return grad, ldg
+
+
+def _distill(where, logits, teacher_ids, teacher_logits, grad_loss, temperature, loss, lse, grad, want_grad):
+    dt, it, tt, ldl, ldi, ldt, n, vocab, k = _distill_args(logits, teacher_ids, teacher_logits, temperature, where)
+    loss = torch.empty(n, dtype=torch.float32, device=logits.device) if loss is None else \
+        _per_row(loss, "loss", n, logits)
+    lse = torch.empty(n, dtype=torch.float32, device=logits.device) if lse is None else _per_row(lse, "lse", n, logits)
+    g_ptr, ldg, gl_ptr = None, 0, None
+    if want_grad:
+        gl_ptr = _per_row(grad_loss, "grad_loss", n, logits).data_ptr()
+        grad, ldg = _grad_like(grad, logits, ldl)
+        g_ptr = grad.data_ptr() or None
+    with _on(logits.device):
+        st = L.load().b2r_topk_distill(
+            loss.data_ptr(), lse.data_ptr(), g_ptr, ldg, gl_ptr, logits.data_ptr(), ldl, dt, teacher_ids.data_ptr(),
+            ldi, it, teacher_logits.data_ptr(), ldt, tt, n, vocab, k, float(temperature),
+            _stream_ptr(logits.device))
+    L.check(st, "b2r_topk_distill")
+    return loss, lse, grad
+
+
+def topk_distill(logits, teacher_ids, teacher_logits, temperature=1.0, loss=None, lse=None):
+    """Distillation loss of every row of student logits against a teacher's top logits:
+
+      p = softmax(teacher_logits / T) over the entries whose token lies in [0, vocab)
+      loss = T^2 * sum_k p_k (log p_k - log softmax(logits / T)[teacher_ids_k]),  lse = log sum exp(logits / T)
+
+    logits: [n_rows x vocab] row-major (rows may be strided), float32 / float16 / bfloat16; teacher_ids: [n_rows x k]
+    int32 / int64, -1 where a list is shorter than k; teacher_logits: [n_rows x k], any of the three types; k <= 1024.
+    A row without a valid entry has loss 0. Returns (loss, lse), float32 vectors."""
+    loss, lse, _ = _distill("topk_distill", logits, teacher_ids, teacher_logits, None, temperature, loss, lse, None,
+                            False)
+    return loss, lse
+
+
+def topk_distill_step(logits, teacher_ids, teacher_logits, grad_loss, temperature=1.0, loss=None, lse=None,
+                      grad=None):
+    """topk_distill and its gradient in one pass over the logits: grad = grad_loss[:, None] * d loss / d logits for
+    a given weight of every row (float32 [n_rows], 1 / n_rows for a mean). `grad` may be `logits`. Returns
+    (loss, lse, grad)."""
+    return _distill("topk_distill_step", logits, teacher_ids, teacher_logits, grad_loss, temperature, loss, lse, grad,
+                    True)
+
+
+def topk_distill_grad(logits, teacher_ids, teacher_logits, lse, grad_loss, temperature=1.0, grad=None):
+    """The gradient of topk_distill alone, from the lse that it returned:
+    grad[r, v] = grad_loss[r] * T * (softmax(logits / T)[r, v] - sum of p_k with teacher_ids[r, k] == v).
+    `grad` may be `logits`. Returns grad."""
+    dt, it, tt, ldl, ldi, ldt, n, vocab, k = _distill_args(logits, teacher_ids, teacher_logits, temperature,
+                                                           "topk_distill_grad")
+    _per_row(lse, "lse", n, logits)
+    _per_row(grad_loss, "grad_loss", n, logits)
+    grad, ldg = _grad_like(grad, logits, ldl)
+    with _on(logits.device):
+        st = L.load().b2r_topk_distill_grad(
+            grad.data_ptr(), ldg, lse.data_ptr(), grad_loss.data_ptr(), logits.data_ptr(), ldl, dt,
+            teacher_ids.data_ptr(), ldi, it, teacher_logits.data_ptr(), ldt, tt, n, vocab, k, float(temperature),
+            _stream_ptr(logits.device))
+    L.check(st, "b2r_topk_distill_grad")
+    return grad
+
+
 def last_kernel_status(device, clear=True):
     """Synchronises `device` and returns L.OK, or L.ERR_TIMEOUT if a bounded wait inside a kernel of any
     earlier call on that device ran out (that call's unfinished floating-point outputs are NaN)."""
