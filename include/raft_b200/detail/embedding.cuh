@@ -51,28 +51,23 @@ lookup_kernel(T* out, int64_t ldo, const T* table, int64_t ldt, const TokT* toke
   const T* src       = table + (valid ? tok : 0) * ldt;
   T* dst             = out + row * ldo;
   const int64_t v0   = int64_t(sg) * (kLookupUnroll << lg) + lane;
-  VecOf<T, V> r[kLookupUnroll];
+  Elems<T, V> r[kLookupUnroll];
 #pragma unroll
   for (int u = 0; u < kLookupUnroll; ++u) {
     const int64_t v = v0 + (int64_t(u) << lg);
-    if (valid && v < nvec) {
-      r[u] = *reinterpret_cast<const VecOf<T, V>*>(src + v * V);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        r[u].e[i] = FloatIo<T>::down(0.0f);
-    }
+    if (valid && v < nvec) r[u].load(src + v * V);
   }
 #pragma unroll
   for (int u = 0; u < kLookupUnroll; ++u) {
     const int64_t v = v0 + (int64_t(u) << lg);
     if (v < nvec) {
-      if (valid) {
+      float f[V];
+      r[u].up(f);
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-          r[u].e[i] = FloatIo<T>::down(FloatIo<T>::up(r[u].e[i]) * scale);
-      }
-      store_vec<T, V>(dst + v * V, r[u]);
+      for (int i = 0; i < V; ++i)
+        f[i] = valid ? f[i] * scale : 0.0f;
+      r[u].down(f);
+      r[u].store(dst + v * V);
     }
   }
   if constexpr (V > 1) {  // the columns behind the last whole vector
@@ -303,18 +298,21 @@ constexpr int kSumBatch   = 8;  // rows a thread has in flight
 template <typename OutT, int V>
 B2R_DI void store_sum(OutT* dst, const float (&acc)[V], float scale, bool accumulate)
 {
-  VecOf<OutT, V> o;
+  Elems<OutT, V> o;
+  float f[V];
   if (accumulate) {
-    o = *reinterpret_cast<const VecOf<OutT, V>*>(dst);
+    o.load(dst);
+    o.up(f);
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      o.e[i] = FloatIo<OutT>::down(fmaf(acc[i], scale, FloatIo<OutT>::up(o.e[i])));
+      f[i] = fmaf(acc[i], scale, f[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      o.e[i] = FloatIo<OutT>::down(acc[i] * scale);
+      f[i] = acc[i] * scale;
   }
-  *reinterpret_cast<VecOf<OutT, V>*>(dst) = o;
+  o.down(f);
+  o.store(dst);
 }
 
 // V fp32 partial sums to or from scratch (16-byte aligned for V = 4, 8)
@@ -383,15 +381,14 @@ sum_rows_kernel(OutT* out, int64_t ldo, float* partial, const InT* g, int64_t ld
       named[threadIdx.x] = lo < n && skey[lo] == v;
     }
     __syncthreads();
-    VecOf<OutT, V> zero;
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      zero.e[i] = FloatIo<OutT>::down(0.0f);
+    Elems<OutT, V> zero;
+    const float zeros[V] = {};
+    zero.down(zeros);
     for (int r = 0; r < rows; ++r) {
       if (named[r]) continue;
       OutT* dst = out + (v0 + r) * ldo;
       for (int64_t v = threadIdx.x; v < nvec; v += kSumThreads)
-        *reinterpret_cast<VecOf<OutT, V>*>(dst + v * V) = zero;
+        zero.store(dst + v * V);
     }
     return;
   }
@@ -412,11 +409,11 @@ sum_rows_kernel(OutT* out, int64_t ldo, float* partial, const InT* g, int64_t ld
     acc[i] = 0.0f;
   for (int64_t i0 = lo; i0 < hi && cur < vocab; i0 += kSumBatch) {
     unsigned key[kSumBatch];
-    VecOf<InT, V> row[kSumBatch];
+    Elems<InT, V> row[kSumBatch];
 #pragma unroll
     for (int u = 0; u < kSumBatch; ++u) {
       key[u] = i0 + u < hi ? skey[i0 + u] : vocab;
-      if (key[u] < vocab) row[u] = load_stream<InT, V>(g + int64_t(spos[i0 + u]) * ldg + col);
+      if (key[u] < vocab) row[u].load_once(g + int64_t(spos[i0 + u]) * ldg + col);
     }
 #pragma unroll
     for (int u = 0; u < kSumBatch; ++u) {
@@ -434,9 +431,11 @@ sum_rows_kernel(OutT* out, int64_t ldo, float* partial, const InT* g, int64_t ld
             acc[i] = 0.0f;
           if (cur >= vocab) break;
         }
+        float f[V];
+        row[u].up(f);
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          acc[i] += FloatIo<InT>::up(row[u].e[i]);
+          acc[i] += f[i];
       }
     }
   }

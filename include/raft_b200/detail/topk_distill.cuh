@@ -14,6 +14,7 @@
 #pragma once
 
 #include "launch.cuh"
+#include "row_normalize_staged.cuh"
 #include "vocab_common.cuh"
 
 #include <cfloat>
@@ -64,6 +65,7 @@ struct Args {
   int vocab;
   double temperature;
   int per_cta;  // vectors of a row per CTA of the cluster
+  RingCtl ctl;  // bounded waits
 };
 
 B2R_DI float ex2(float x)
@@ -96,66 +98,112 @@ B2R_DI void cluster_store(float2* p, unsigned rank, float2 v)
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(remote), "f"(v.x), "f"(v.y) : "memory");
 }
 
-B2R_DI void cluster_store_f64(double* p, unsigned rank, double v)
+// 16 bytes to the same place of CTA `rank`, counted by the barrier at the same place there: the data has arrived when
+// the barrier's phase completes. No fence is involved, so global stores under way are not waited for.
+B2R_DI void cluster_send(float4* p, uint64_t* bar, unsigned rank, float4 v)
 {
-  const unsigned local = unsigned(__cvta_generic_to_shared(p));
-  unsigned remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
-  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(remote), "d"(v) : "memory");
+  unsigned to, at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(at)
+               : "memory");
 }
 
-// One row as 16-byte vectors of its memory: vector j holds elements [j * VE - phase, (j + 1) * VE - phase), where
-// `phase` elements lie between the 16-byte boundary at or before the row's first element and that element. Only
-// whole vectors are moved as vectors; the elements of the first and last one are moved one by one, so nothing
-// outside the row is touched.
+B2R_DI void cluster_send(double* p, uint64_t* bar, unsigned rank, double v)
+{
+  unsigned to, at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to),
+               "l"(__double_as_longlong(v)), "r"(at)
+               : "memory");
+}
+
+// A part of a row as 16-byte vectors of its memory. Vector j of a row holds elements [j * VE - phase, (j + 1) * VE -
+// phase), where `phase` elements lie between the 16-byte boundary at or before the row's first element and that
+// element. Only whole vectors are moved as vectors: the first vector of a row and its last may not be, their elements
+// are moved one by one, so nothing outside the row is touched.
 template <typename T>
-struct RowVecs {
+struct RowPart {
   static constexpr int VE = Vec16Of<T>::value;
-  int phase, vocab, n;  // n vectors
+  const T* at;     // where element 0 of the part's first vector is, or would be
+  int first;       // its token (negative: before the row)
+  int n;           // vectors of the part
+  int lo, hi;      // those that are whole: [lo, hi)
+  int token0, token1;  // tokens of the part
 
-  B2R_DI RowVecs(const T* row, int v)
+  // vectors [j0, j0 + most) of the row
+  B2R_DI RowPart(const T* row, int vocab, int j0, int most) : RowPart(row, phase_of(row), vocab, j0, most) {}
+  B2R_DI static int phase_of(const T* row) { return int(uintptr_t(row) & 15u) / int(sizeof(T)); }
+  B2R_DI RowPart(const T* row, int phase, int vocab, int j0, int most)
   {
-    phase = int((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-    vocab = v;
-    n     = (phase + v + VE - 1) / VE;
+    const int end   = phase + vocab;  // behind the row, in elements from the boundary
+    const int all   = (end + VE - 1) / VE;
+    n               = all - j0 < most ? (all > j0 ? all - j0 : 0) : most;
+    first           = j0 * VE - phase;
+    at              = row + first;
+    lo              = first < 0 && n > 0 ? 1 : 0;
+    hi              = n - (n > 0 && j0 + n == all && end % VE != 0 ? 1 : 0);
+    token0          = first > 0 ? first : 0;
+    token1          = first + n * VE < vocab ? first + n * VE : vocab;
   }
-  B2R_DI int first(int j) const { return j * VE - phase; }  // element index of lane 0 of vector j
-  B2R_DI bool whole(int j) const { return first(j) >= 0 && first(j) + VE <= vocab; }
+  B2R_DI bool whole(int i) const { return i >= lo && i < hi; }
+  B2R_DI bool edges() const { return lo != 0 || hi < n; }
 
-  B2R_DI VecOf<T, VE> load(const T* row, int j) const
+  B2R_DI Words4 load_whole(int i) const
   {
-    VecOf<T, VE> r;
-    if (j < n && whole(j)) {
-      uint32_t w[4];  // not the non-coherent path: the gradient may be written over the logits
-      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                   : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                   : "l"(row + first(j))
-                   : "memory");
-      memcpy(&r, w, 16);
-      return r;
-    }
+    Words4 r;
+    // not the non-coherent path: the gradient may be written over the logits
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3])
+                 : "l"(at + i * VE)
+                 : "memory");
+    return r;
+  }
+  // a vector that may reach over an end of the row: -inf there
+  B2R_DI Words4 load_edge(int i) const
+  {
+    Words4 r;
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const int e = first(j) + i;
-      r.e[i]      = j < n && e >= 0 && e < vocab ? row[e] : FloatIo<T>::down(-INFINITY);
+    for (int e = 0; e < VE; ++e) {
+      const int t = first + i * VE + e;
+      put_bits<T>(r, e, t >= token0 && t < token1 ? at[i * VE + e] : FloatIo<T>::down(-INFINITY));
     }
     return r;
   }
-  // `same`: the row of `dst` has the same phase
-  B2R_DI void store(T* dst, int j, const VecOf<T, VE>& v, bool same) const
+  B2R_DI Words4 load(int i) const { return whole(i) ? load_whole(i) : load_edge(i); }
+  // element by element, as much of it as belongs to the part; `dst` where `at` is in the output's row
+  B2R_DI void store_edge(T* dst, int i, const Words4& v) const
   {
-    if (j >= n) return;
-    if (same && whole(j)) {
-      store_vec<T, VE>(dst + first(j), v);
-      return;
-    }
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const int e = first(j) + i;
-      if (e >= 0 && e < vocab) dst[e] = v.e[i];
+    for (int e = 0; e < VE; ++e) {
+      const int t = first + i * VE + e;
+      if (t >= token0 && t < token1) dst[i * VE + e] = get_bits<T>(v, e);
     }
   }
+  // `same`: the output's row has the same phase
+  B2R_DI void store(T* dst, int i, const Words4& v, bool same) const
+  {
+    if (same && whole(i))
+      *reinterpret_cast<Words4*>(dst + i * VE) = v;
+    else
+      store_edge(dst, i, v);
+  }
 };
+template <typename T>
+B2R_DI Words4 minus_inf()
+{
+  Words4 r;
+#pragma unroll
+  for (int q = 0; q < Vec16Of<T>::value / 2; ++q)
+    down_pair<T>(r, q, make_float2(-INFINITY, -INFINITY));
+  return r;
+}
+B2R_DI bool same_phase(const void* a, const void* b)
+{
+  return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15u) == 0;
+}
 
 // 16 bytes from global to shared memory, asynchronous (the thread's own commit / wait groups order it)
 B2R_DI void copy_async16(void* smem, const void* g)
@@ -170,13 +218,71 @@ B2R_DI void copy_wait()
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// NaN operands lose, as in fmaxf
 B2R_DI float warp_max(float v)
 {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
-  return v;
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
+B2R_DI float max3(float a, float b, float c)
+{
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// Two fp32 values handled by one instruction.
+using Pair = unsigned long long;
+B2R_DI Pair pair(float a, float b)
+{
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+B2R_DI float2 split(Pair p)
+{
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+B2R_DI Pair add2(Pair a, Pair b)
+{
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+B2R_DI Pair mul2(Pair a, Pair b)
+{
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+B2R_DI Pair fma2(Pair a, Pair b, Pair c)
+{
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+// 2^x of both
+B2R_DI Pair ex2_2(Pair x)
+{
+  const float2 v = split(x);
+  return pair(ex2(v.x), ex2(v.y));
+}
+
+template <typename T>
+B2R_DI Pair up2(const Words4& v, int q)
+{
+  const float2 f = up_pair<T>(v, q);
+  return pair(f.x, f.y);
+}
+template <typename T>
+B2R_DI void down2(Words4& v, int q, Pair p)
+{
+  down_pair<T>(v, q, split(p));
+}
+
 template <typename F>
 B2R_DI F warp_sum(F v)
 {
@@ -236,15 +342,20 @@ B2R_DI bool weigh_list(const int* id, float* y, int k, float inv_t)
   return some;
 }
 
-// Entry j of a row's list as weigh_list wants it.
-template <typename T>
-B2R_DI void fetch_entry(const Args<T>& a, int64_t row, int j, int* id, float* y)
-{
-  const int64_t t = a.list.id(row, j);
-  const bool ok   = t >= 0 && t < a.vocab;
-  *id             = ok ? int(t) : -1;
-  *y              = ok ? a.list.logit(row, j) : -INFINITY;
-}
+// Entry j of a row's list. Both loads are under way before either value is looked at.
+struct Entry {
+  int64_t token;
+  float y;
+
+  template <typename T>
+  B2R_DI void ask(const Args<T>& a, int64_t row, int j)
+  {
+    token = a.list.id(row, j);
+    y     = a.list.logit(row, j);
+  }
+  // as weigh_list wants it
+  B2R_DI int id(int vocab) const { return token >= 0 && token < vocab ? int(token) : -1; }
+};
 
 // Weight of entry j's token over the whole list (a token may be named more than once); false unless j is the first
 // entry of its token, which speaks for all of them.
@@ -265,233 +376,368 @@ B2R_DI bool listed_weight(const int* id, const float* logp, int k, int j, float*
 
 // ---------------------------------------------------------------------------------------
 // Loss and gradient in one pass. A cluster takes a row, every CTA of it `per_cta` vectors; clusters are persistent and
-// walk the rows. Every thread copies its own vectors of the rows to come into shared memory (two rows ahead, kStages
-// buffers), so that the memory system is busy while a row is worked on, and nobody has to wait for anybody to use
-// them. A thread turns its elements into exponentials relative to its own maximum and keeps those in registers; ONE
-// cluster barrier per row carries the (m, s) of every warp to every CTA, after which the gradient is a product per
-// element. One exponential per element: at two the MUFU unit (16 per clock and SM) would bound the kernel.
+// walk the rows. Rows come into a ring of kStages shared-memory buffers by bulk copies; the workers go over a row twice
+// there. The first time each takes (m, s) of its elements; the CTA's (m, s) goes to every CTA of the cluster as a record
+// that a shared-memory barrier counts. The second time they write the gradient over the row, and a bulk copy takes it
+// to memory. Between the two lies the first pass over the NEXT row, so that nobody waits for the records.
 //
-// Everything that hangs on the list runs beside that, a step ahead or behind, so that its chains of dependent loads
-// are off the path: entries are loaded two rows ahead, their softmax is taken one row ahead by one warp, the student
-// logits of listed tokens are read from the buffers of the CTA that holds them, and the listed elements of the
-// gradient are written one barrier after the vectors they lie in (the barrier orders the two writes).
+// Two exponentials per element: 8 elements per clock and SM at the MUFU unit's 16, 4100 clocks of a row's 64 KB part,
+// against 5100 that its 128 KB of traffic take. Keeping the first pass's exponentials instead needs 64 registers of
+// every worker for them; ptxas then spills (512 workers of 64 elements: 96 registers, 815 us for 4096 rows of 131072
+// bf16; 256 of 128: 168 registers, 1195 us). Forms before that: workers that copied their own vectors in and out, 750 us
+// (5000 of 12000 clocks per row in the copies); cluster barriers for the exchange, which wait for the gradient's
+// stores, 1350 us.
+//
+// Two warps work beside the workers, so that no chain of loads is on the workers' path:
+//   the sender   joins the CTA's (m, s), sends the record, issues the copies, and in the first CTA writes the loss;
+//   the lister   prepares the list of the row after the next: weights, the student's logits of the listed tokens, and
+//                the sums A = sum p (log p - z / T), P = sum p over the tokens this CTA holds, of which the loss is
+//                T^2 (A + P lse). (The listed elements of the gradient are written by the warp that holds them.)
+//
+// kEven: all rows have the phase of the first, so that the geometry is worked out once.
 // ---------------------------------------------------------------------------------------
-constexpr int kStages = 3;
-constexpr int kStepNv = 4;
+constexpr int kStages = 3;  // vectors of the row in its second pass, of the next in its first, of the one after under way
+constexpr int kStepNv = 8;  // vectors of a worker, in chunks of four
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT)
+template <typename T, int NT, bool kEven>
+__global__ void __launch_bounds__(NT + 64)
 distill_step_kernel(const Args<T> a)
 {
   constexpr int VE = Vec16Of<T>::value;
   constexpr int NV = kStepNv;
   constexpr int NW = NT / 32;
-  using Vec        = VecOf<T, VE>;
-  extern __shared__ __align__(16) unsigned char step_smem[];
-  __shared__ float2 parts[2][8 * NW];   // (m, s) of every warp of the cluster, by CTA rank
-  __shared__ double loss_part[2][8];    // rank 0: the loss sums of the CTAs
+  constexpr int CV = 4;            // vectors of a chunk
+  constexpr int CP = CV * VE / 2;  // pairs of a chunk
+  using Vec        = Words4;
+  extern __shared__ __align__(128) unsigned char step_smem[];
+  // Records by row & 3: a CTA that is ahead may send the row after the next while another still reads the row before.
+  __shared__ __align__(16) float4 record[4][8];   // by CTA rank: m, s, A (fp64)
+  __shared__ __align__(8) double record_p[4][8];  // P
+  __shared__ __align__(8) uint64_t arrived[4];
+  __shared__ __align__(8) uint64_t full[kStages];
+  __shared__ float2 warp_part[NW];
+  __shared__ double list_sums[3][2];  // A, P
+  __shared__ float factor_s[3];       // weight of the row's gradient, 0 for a row without a list
   __shared__ int some_s[3];
-  Vec* stages   = reinterpret_cast<Vec*>(step_smem);             // [kStages][NT * NV]
-  const int k   = a.list.k;
-  int* ids      = reinterpret_cast<int*>(stages + kStages * NT * NV);  // [3][k]
-  float* logps  = reinterpret_cast<float*>(ids + 3 * k);               // [3][k]
-  int* late_id  = reinterpret_cast<int*>(logps + 3 * k);               // [k] token whose element is still to be written
-  float* late_v = reinterpret_cast<float*>(late_id + k);               // [k]
+  __shared__ int gave_up;
+  Vec* stages         = reinterpret_cast<Vec*>(step_smem);                   // [kStages][NT * NV]
+  const int k         = a.list.k;
+  int* ids            = reinterpret_cast<int*>(stages + kStages * NT * NV);  // [3][k]
+  float* logps        = reinterpret_cast<float*>(ids + 3 * k);               // [3][k]
+  float* zids         = logps + 3 * k;                                       // [3][k]
   const unsigned rank = cluster_rank();
   const unsigned size = cluster_size();
   const int tid       = int(threadIdx.x);
   const int warp = tid >> 5, lane = tid & 31;
-  cluster_arrive();  // every CTA of the cluster has started: waited for before the first remote store
-  grid_dep_sync();
-
+  if (tid == 0) {
+    for (int i = 0; i < 4; ++i)
+      mbar_init(&arrived[i], 1);
+    for (int i = 0; i < kStages; ++i)
+      mbar_init(&full[i], 1);
+    gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
   const int64_t step  = int64_t(gridDim.x) / size;
   const int64_t first = int64_t(blockIdx.x) / size;
   const float c       = float(1.4426950408889634 / a.temperature);
-  const float inv_t   = float(1.0 / a.temperature);
   const int j0        = int(rank) * a.per_cta;
+  const auto part_of  = [&](int64_t row) {
+    const T* z = a.logits + row * a.ldl;
+    return RowPart<T>(z, RowPart<T>::phase_of(kEven ? a.logits : z), a.vocab, j0, a.per_cta);
+  };
+  // Places behind the end of a part hold -inf, which adds nothing: no vector has to be asked about when it is used.
+  // Nobody writes there again, but for rows of different phases, whose parts differ by a vector.
+  {
+    const RowPart<T> part = part_of(0);
+    for (int i = tid; i < NT * NV; i += NT + 64)
+      if (i >= part.n) stages[i] = stages[NT * NV + i] = stages[2 * NT * NV + i] = minus_inf<T>();
+  }
+  fence_proxy_async();
+  __syncthreads();
+  cluster_arrive();  // every CTA of the cluster has started, its barriers are set up
+  grid_dep_sync();
 
-  // the thread's vectors of a row on their way into buffer `stage`
+  // ---- sender
+  // row's vectors on their way into buffer `stage` (all lanes of the warp come here)
   auto request = [&](int64_t row, int stage) {
-    if (row < a.n_rows) {
-      const T* z = a.logits + row * a.ldl;
-      const RowVecs<T> rv(z, a.vocab);
-      const int j1 = j0 + a.per_cta < rv.n ? j0 + a.per_cta : rv.n;
+    if (row >= a.n_rows) return;
+    const RowPart<T> part = part_of(row);
+    Vec* to               = stages + stage * (NT * NV);
+    if (lane == 0) {
+      const int whole = part.hi > part.lo ? part.hi - part.lo : 0;
+      mbar_expect_tx(&full[stage], unsigned(whole) * 16u);
+      for (int i = 0; i < whole; i += 1024) {
+        const int n = whole - i < 1024 ? whole - i : 1024;
+        bulk_load(to + part.lo + i, part.at + (part.lo + i) * VE, unsigned(n) * 16u, &full[stage]);
+      }
+      if (part.lo != 0) to[0] = part.load_edge(0);
+    }
+    if (lane == 1 && part.hi < part.n && (part.n > 1 || part.lo == 0)) to[part.n - 1] = part.load_edge(part.n - 1);
+    if (!kEven && lane == 2 && part.n < NT * NV) to[part.n] = minus_inf<T>();
+  };
+  // the gradient of a row from its buffer to memory, as far as that goes in whole vectors
+  auto write_back = [&](int64_t row, int stage) {
+    const RowPart<T> part = part_of(row);
+    T* g                  = a.grad + row * a.ldg;
+    if (lane == 0 && part.hi > part.lo && same_phase(g, a.logits + row * a.ldl))
+      bulk_store(g + part.first + part.lo * VE, stages + stage * (NT * NV) + part.lo, unsigned(part.hi - part.lo) * 16u);
+  };
+  // the record of a row whose parts the workers have left in warp_part (all lanes); n: the row's number here
+  auto send = [&](int n, int buf) {
+    const float2 v = lane < NW ? warp_part[lane] : make_float2(-INFINITY, 0.0f);
+    const ExpSum w = warp_join({v.x, v.y}, c);
+    const long long bits = __double_as_longlong(list_sums[buf][0]);
+    const float4 rec = make_float4(w.m, w.s, __int_as_float(int(bits)), __int_as_float(int(bits >> 32)));
+    const int at     = n & 3;
+    const bool skip  = blockIdx.x == 0 && n == a.ctl.skip_tile;  // test hook: this record is never sent
+    if (size == 1) {
+      if (lane == 0 && !skip) {
+        record[at][0]   = rec;
+        record_p[at][0] = list_sums[buf][1];
+        mbar_arrive(&arrived[at]);
+      }
+    } else {
+      if (lane == 0) mbar_expect_tx(&arrived[at], size * 24u);
+      if (lane < int(size) && !skip) {
+        cluster_send(&record[at][rank], &arrived[at], unsigned(lane), rec);
+        cluster_send(&record_p[at][rank], &arrived[at], unsigned(lane), list_sums[buf][1]);
+      }
+    }
+  };
+
+  // ---- lister
+  const double inverse = 1.0 / a.temperature;
+  auto prepare         = [&](int64_t row, int buf, int stage, unsigned phase) {
+    if (row >= a.n_rows) return;
+    const RowPart<T> part = part_of(row);
+    const float weight    = a.grad_loss[row];
+    int* id               = ids + buf * k;
+    float* logp           = logps + buf * k;
+    float* zid            = zids + buf * k;
+    for (int l0 = 0; l0 < k; l0 += 128) {
+      Entry entry[4];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = j0 + i * NT + tid;
-        if (j < j1) {
-          Vec* to = stages + stage * (NT * NV) + i * NT + tid;
-          if (rv.whole(j))
-            copy_async16(to, z + rv.first(j));
-          else
-            *to = rv.load(z, j);
+      for (int u = 0; u < 4; ++u)
+        if (l0 + u * 32 + lane < k) entry[u].ask(a, row, l0 + u * 32 + lane);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = l0 + u * 32 + lane;
+        if (j < k) {
+          id[j]   = entry[u].id(a.vocab);
+          logp[j] = entry[u].y;
         }
       }
     }
-    copy_commit();
-  };
-  // entry `tid` of a row's list in registers (lists longer than the CTA: the rest is fetched where it is stored)
-  int next_id  = -1;
-  float next_y = 0.0f;
-  auto ask_list = [&](int64_t row) {
-    if (row < a.n_rows && tid < k) fetch_entry(a, row, tid, &next_id, &next_y);
-  };
-  auto store_list = [&](int64_t row, int buf) {
-    if (row >= a.n_rows) return;
-    if (tid < k) {
-      ids[buf * k + tid]   = next_id;
-      logps[buf * k + tid] = next_y;
+    const bool some = weigh_list(id, logp, k, float(inverse));
+    // the row itself, for the student's logits of the listed tokens
+    const bool here = mbar_wait_bounded(&full[stage], phase, &gave_up, a.ctl.limit_ns);
+    const T* held   = reinterpret_cast<const T*>(stages + stage * (NT * NV)) - part.first;  // held[t]: token t
+    double sum = 0.0, share = 0.0;
+    for (int j = lane; j < k && some && here; j += 32) {
+      const int t    = id[j];
+      const float lp = logp[j];
+      if (t >= part.token0 && t < part.token1) {
+        const float z  = FloatIo<T>::up(held[t]);
+        const double w = double(expf(lp));
+        zid[j]         = z;
+        sum += lp == -INFINITY ? 0.0 : w * (double(lp) - double(z) * inverse);
+        share += w;
+      }
     }
-    for (int j = tid + NT; j < k; j += NT)
-      fetch_entry(a, row, j, &ids[buf * k + j], &logps[buf * k + j]);
+    sum   = warp_sum(sum);
+    share = warp_sum(share);
+    if (lane == 0) {
+      list_sums[buf][0] = here ? sum : double(NAN);
+      list_sums[buf][1] = share;
+      some_s[buf]       = some;
+      factor_s[buf]     = some ? float(double(weight) * a.temperature) : 0.0f;
+    }
   };
-  for (int j = tid; j < k; j += NT)
-    late_id[j] = -1;
 
-  request(first, 0);
-  request(first + step, 1);
-  ask_list(first);
-  store_list(first, 0);
-  ask_list(first + step);
-  __syncthreads();
-  if (warp == NW - 1 && first < a.n_rows) {
-    const bool some = weigh_list(ids, logps, k, inv_t);
-    if (lane == 0) some_s[0] = some;
-  }
-  cluster_wait();
-
-  int64_t late_row = -1;  // row whose listed elements and loss are still to be written
-  int stage        = 0;   // it % kStages == it % 3: buffer of the row's vectors and of its list
-  double my_loss   = 0.0;
-  float late_lse   = 0.0f;
-  int par          = 0;   // it & 1
-  for (int64_t row = first;; row += step, par ^= 1) {
-    const bool on       = row < a.n_rows;  // the last turn only finishes what is late
-    const int stage1    = stage + 1 == kStages ? 0 : stage + 1;
-    const T* z          = a.logits + (on ? row : 0) * a.ldl;
-    const RowVecs<T> rv(z, a.vocab);
-    const int j1        = j0 + a.per_cta < rv.n ? j0 + a.per_cta : rv.n;
-    store_list(row + step, stage1);
-    ask_list(row + 2 * step);
+  // ---- workers
+  bool there = true;  // everything waited for so far has arrived
+  // (m, s) of the warp's elements of the row in buffer `stage`
+  auto first_pass = [&](int n, int stage, unsigned phase) {
+    there = there && mbar_wait_bounded(&full[stage], phase, &gave_up, a.ctl.limit_ns);
     const Vec* mine = stages + stage * (NT * NV) + tid;
-    float e[NV * VE];
-    float m = -INFINITY;
-    if (on) {
-      copy_wait<1>();
+    float m = -INFINITY, s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (j0 + i * NT + tid < j1) {
-          const Vec v = mine[i * NT];
+    for (int i0 = 0; i0 < NV; i0 += CV) {
+      if (i0 * NT + warp * 32 >= n) break;
+      Pair e[CP];
+      float top = m;
 #pragma unroll
-          for (int q = 0; q < VE; ++q) {
-            e[i * VE + q] = FloatIo<T>::up(v.e[q]);
-            m             = fmaxf(m, e[i * VE + q]);
-          }
-        } else {
+      for (int i = 0; i < CV; ++i) {
+        const Vec v = mine[(i0 + i) * NT];
 #pragma unroll
-          for (int q = 0; q < VE; ++q)
-            e[i * VE + q] = -INFINITY;
+        for (int q = 0; q < VE / 2; ++q) {
+          e[i * VE / 2 + q] = up2<T>(v, q);
+          const float2 f    = split(e[i * VE / 2 + q]);
+          top               = max3(top, f.x, f.y);
         }
+      }
+      if (top > m) {
+        s = m == -INFINITY ? s : s * ex2((m - top) * c);
+        m = top;
       }
       const float base = m == -INFINITY ? 0.0f : m;
-      float s          = 0.0f;
+      const Pair sub = pair(-base, -base), mul = pair(c, c);
+      Pair sum0 = pair(s, 0.0f), sum1 = pair(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (j0 + i * NT < j1) {
+      for (int q = 0; q < CP; q += 2) {
+        sum0 = add2(sum0, ex2_2(mul2(add2(e[q], sub), mul)));
+        sum1 = add2(sum1, ex2_2(mul2(add2(e[q + 1], sub), mul)));
+      }
+      const float2 s2 = split(add2(sum0, sum1));
+      s               = s2.x + s2.y;
+    }
+    const ExpSum w = warp_join({m, s}, c);
+    if (lane == 0) warp_part[warp] = make_float2(w.m, w.s);
+  };
+  // the gradient of the row in buffer `stage`, written over it (vectors that are not whole, or whose row in memory has
+  // another phase: straight to memory, an element at a time)
+  auto second_pass = [&](int64_t row, int n, int buf, int stage, unsigned phase) {
+    there            = there && mbar_wait_bounded(&arrived[n & 3], phase, &gave_up, a.ctl.limit_ns);
+    const float4 r   = lane < int(size) ? record[n & 3][lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    ExpSum all       = warp_join({r.x, r.y}, c);
+    if (!there) all.s = NAN;
+    const bool some  = some_s[buf] != 0;
+    const float fact = factor_s[buf];
+    const float l2s  = log2f(all.s);
+    const Pair sub = pair(-all.m, -all.m), mul = pair(c, c), off = pair(-l2s, -l2s), fact2 = pair(fact, fact);
+    const RowPart<T> part = part_of(row);
+    Vec* mine             = stages + stage * (NT * NV) + tid;
+    T* to                 = a.grad + row * a.ldg + part.first;
+    const bool same       = same_phase(to, part.at);
+    const bool plain      = same && !part.edges();  // nothing goes straight to memory
 #pragma unroll
-          for (int q = 0; q < VE; ++q) {
-            e[i * VE + q] = ex2((e[i * VE + q] - base) * c);
-            s += e[i * VE + q];
+    for (int i = 0; i < NV; ++i) {
+      if (i * NT + warp * 32 < part.n) {
+        const Vec v = mine[i * NT];
+        Vec o;
+#pragma unroll
+        for (int q = 0; q < VE / 2; ++q)
+          down2<T>(o, q, mul2(ex2_2(fma2(add2(up2<T>(v, q), sub), mul, off)), fact2));
+        if (!some) o = Vec{};
+        const int j = i * NT + tid;
+        if (part.whole(j)) mine[i * NT] = o;
+        if (!plain && j < part.n && !(same && part.whole(j))) part.store_edge(to, j, o);
+      }
+    }
+    // the listed elements of the warp's vectors: q - sum of the token's weights
+    __syncwarp();
+    if (some) {
+      const int* id     = ids + buf * k;
+      const float* logp = logps + buf * k;
+      const float* zid  = zids + buf * k;
+      for (int l0 = 0; l0 < k; l0 += 32) {
+        const int t0  = l0 + lane < k ? id[l0 + lane] : -1;
+        const bool my = t0 >= part.token0 && t0 < part.token1 && (unsigned(t0 - part.first) / VE) % NT / 32 == unsigned(warp);
+        for (unsigned left = __ballot_sync(kFull, my); left != 0u; left &= left - 1u) {
+          const int j = l0 + __ffs(int(left)) - 1;
+          const int t = id[j];
+          float w     = 0.0f;
+          int before  = 0;  // entries of the token ahead of this one: the first speaks for all
+          for (int i = lane; i < k; i += 32) {
+            if (id[i] == t) {
+              w += expf(logp[i]);
+              before += i < j;
+            }
+          }
+          w = warp_sum(w);
+          if (!__any_sync(kFull, before != 0) && lane == 0) {
+            const T v    = FloatIo<T>::down(fact * (ex2((zid[j] - all.m) * c - l2s) - w));
+            const int at = t - part.first;
+            if (same && part.whole(at / VE))
+              reinterpret_cast<T*>(stages + stage * (NT * NV))[at] = v;
+            else
+              to[at] = v;
           }
         }
       }
-      const ExpSum w = warp_join({m, s}, c);
-      if (lane < int(size)) cluster_store(&parts[par][rank * NW + warp], unsigned(lane), make_float2(w.m, w.s));
     }
-    if (late_row >= 0 && warp == 0 && lane == 0) cluster_store_f64(&loss_part[par][rank], 0, my_loss);
-    cluster_arrive();
-    cluster_wait();
+    fence_proxy_async();
+  };
 
-    if (late_row >= 0) {
-      T* g = a.grad + late_row * a.ldg;
-      for (int j = tid; j < k; j += NT) {
-        if (late_id[j] >= 0) g[late_id[j]] = FloatIo<T>::down(late_v[j]);
-        late_id[j] = -1;
-      }
-      if (rank == 0 && tid == 0) {
-        double sum = 0.0;
-        for (unsigned r = 0; r < size; ++r)
-          sum += loss_part[par][r];
-        if (a.loss != nullptr) a.loss[late_row] = float(sum * a.temperature * a.temperature);
-        if (a.lse != nullptr) a.lse[late_row] = late_lse;
-      }
-    }
-    if (!on) break;
-    request(row + 2 * step, stage == 0 ? kStages - 1 : stage - 1);
+  // Row number n of this cluster lies in buffer n % 3, as does its list; its records at n & 3.
+  if (warp == NW) {
+    for (int n = 0; n < kStages; ++n)
+      request(first + n * step, n);
+  }
+  __syncthreads();
+  if (warp == NW + 1) prepare(first, 0, 0, 0);
+  if (warp == NW + 1) prepare(first + step, 1, 1, 0);
+  if (warp < NW) first_pass(part_of(first).n, 0, 0);
+  cluster_wait();
+  __syncthreads();
+  if (warp == NW) send(0, 0);
 
-    const ExpSum all   = join_parts(parts[par], int(size) * NW, c);
-    const float l2s    = log2f(all.s);
-    const bool some    = some_s[stage] != 0;
-    const float factor = some ? float(double(a.grad_loss[row]) * a.temperature) : 0.0f;
-    // a thread without a maximum holds zeros (or NaN)
-    const float scale = (m == -INFINITY ? (all.s > 0.0f ? 0.0f : NAN) : ex2((m - all.m) * c - l2s)) * factor;
-    T* g               = a.grad + row * a.ldg;
-    const bool same    = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int j = j0 + i * NT + tid;
-      if (j < j1) {
-        Vec o;
-#pragma unroll
-        for (int q = 0; q < VE; ++q)
-          o.e[q] = FloatIo<T>::down(some ? e[i * VE + q] * scale : 0.0f);
-        rv.store(g, j, o, same);
-      }
-    }
-    // the list's part
-    const int* id     = ids + stage * k;
-    const float* logp = logps + stage * k;
-    const T* held     = reinterpret_cast<const T*>(stages + stage * (NT * NV)) - rv.first(j0);  // held[t]: token t
-    const int lo      = rv.first(j0) > 0 ? rv.first(j0) : 0;
-    const int hi      = rv.first(j1) < a.vocab ? rv.first(j1) : a.vocab;
-    if (some) {
-      for (int j = tid; j < k; j += NT) {
-        const int t = id[j];
-        float w;
-        if (t >= lo && t < hi && listed_weight(id, logp, k, j, &w)) {
-          late_id[j] = t;
-          late_v[j]  = factor * (ex2((FloatIo<T>::up(held[t]) - all.m) * c - l2s) - w);
+  int cur        = 0;   // n % 3, and the parity of its round
+  unsigned round = 0;
+  int n          = 0;
+  for (int64_t row = first; row < a.n_rows; row += step, ++n) {
+    const int nxt         = cur + 1 == kStages ? 0 : cur + 1;
+    const unsigned nround = nxt == 0 ? round ^ 1u : round;
+    const int nn          = nxt + 1 == kStages ? 0 : nxt + 1;
+    const unsigned phase  = unsigned(n >> 2) & 1u;  // of the records
+    if (warp < NW && row + step < a.n_rows) first_pass(part_of(row + step).n, nxt, nround);
+    __syncthreads();
+    if (warp < NW) {
+      second_pass(row, n, cur, cur, phase);
+    } else if (warp == NW) {
+      if (row + step < a.n_rows && there) send(n + 1, nxt);
+      there = there && mbar_wait_bounded(&arrived[n & 3], phase, &gave_up, a.ctl.limit_ns);
+      if (rank == 0) {
+        const float4 r   = lane < int(size) ? record[n & 3][lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        const double p   = lane < int(size) ? record_p[n & 3][lane] : 0.0;
+        const ExpSum all = warp_join({r.x, r.y}, c);
+        const double sum = warp_sum(__longlong_as_double((long long)(unsigned(__float_as_int(r.z))) |
+                                                         ((long long)(__float_as_int(r.w)) << 32)));
+        const double wgt = warp_sum(p);
+        const double lse = there ? double(all.m) * inverse + double(logf(all.s)) : double(NAN);
+        if (lane == 0) {
+          if (a.loss != nullptr)
+            a.loss[row] = some_s[cur] != 0 ? float((sum + wgt * lse) * a.temperature * a.temperature) : 0.0f;
+          if (a.lse != nullptr) a.lse[row] = float(lse);
         }
       }
+    } else if (there) {
+      // (the buffer of this row's successor's successor: its list goes where the row before had its)
+      prepare(row + 2 * step, nn, nn, nn == 0 || nxt == 0 ? round ^ 1u : round);
     }
-    if (warp == 0) {
-      const double lse = double(all.m) / a.temperature + double(logf(all.s));
-      double sum       = 0.0;
-      for (int j = lane; j < k && some; j += 32) {
-        const int t    = id[j];
-        const float lp = logp[j];
-        if (t >= lo && t < hi && !(lp == -INFINITY))
-          sum += double(expf(lp)) * (double(lp) - (double(FloatIo<T>::up(held[t])) / a.temperature - lse));
-      }
-      my_loss  = warp_sum(sum);
-      late_lse = float(lse);
+    __syncthreads();
+    if (warp == NW) {
+      write_back(row, cur);
+      bulk_store_wait_read();  // (by the lane that stores)
+      __syncwarp();
+      // (after a give-up nothing says that the buffer's last copy has landed)
+      if (there && *static_cast<volatile int*>(&gave_up) == 0) request(row + 3 * step, cur);
     }
-    if (warp == NW - 1 && row + step < a.n_rows) {
-      const bool next = weigh_list(ids + stage1 * k, logps + stage1 * k, k, inv_t);
-      if (lane == 0) some_s[stage1] = next;
-    }
-    late_row = row;
-    stage    = stage1;
+    cur   = nxt;
+    round = nround;
   }
-  copy_wait<0>();
+  if (warp == NW) {
+    bulk_store_wait_all();
+    if (*static_cast<volatile int*>(&gave_up) != 0 && lane == 0) {
+      // copies still on their way in must have landed before the CTA leaves: the last of each buffer, if any
+      for (int i = 0; i < kStages; ++i)
+        (void)mbar_drain_bounded(&full[i], i < cur ? round : round ^ 1u, a.ctl.limit_ns);
+    }
+  }
+  if (!there && tid == 0) ring_report_timeout(a.ctl);
+  if (size > 1) {  // nobody sends to a CTA that has left
+    cluster_arrive();
+    cluster_wait();
+  }
 }
 
 // ---------------------------------------------------------------------------------------
 // Rows that do not fit the registers of a cluster (kGrad), and the loss alone: NT threads stream their CTA's part of
-// the row, the next vectors under way while these are worked on, and one more warp of rank 0's CTA takes the list.
-// With kGrad every part is read a second time.
+// the row through shared memory (every thread its own vectors, kStreamDepth - 1 chunks of kStreamNv vectors under way),
+// and one more warp of rank 0's CTA takes the list. With kGrad every part is read a second time.
 // ---------------------------------------------------------------------------------------
-constexpr int kStreamNv = 4;
+constexpr int kStreamNv    = 8;
+constexpr int kStreamDepth = 3;
 
 template <typename T, int NT, bool kGrad>
 __global__ void __launch_bounds__(NT + 32)
@@ -500,7 +746,7 @@ distill_stream_kernel(const Args<T> a)
   constexpr int VE = Vec16Of<T>::value;
   constexpr int NV = kStreamNv;
   constexpr int NW = NT / 32;
-  using Vec        = VecOf<T, VE>;
+  using Vec        = Words4;
   extern __shared__ __align__(16) unsigned char stream_smem[];
   __shared__ float2 parts[8 * NW];
   __shared__ int some_s;
@@ -509,22 +755,25 @@ distill_stream_kernel(const Args<T> a)
   const int tid       = int(threadIdx.x);
   const int warp = tid >> 5, lane = tid & 31;
   const int k   = a.list.k;
-  int* id       = reinterpret_cast<int*>(stream_smem);  // [k]
+  Vec* ring     = reinterpret_cast<Vec*>(stream_smem);                 // [kStreamDepth][NT * NV]
+  int* id       = reinterpret_cast<int*>(ring + kStreamDepth * NT * NV);  // [k]
   float* logp   = reinterpret_cast<float*>(id + k);     // [k]
   float* zid    = logp + k;                             // [k] student logits of the listed tokens
   cluster_arrive();
   grid_dep_sync();
   const int64_t row = int64_t(blockIdx.x) / size;
   const T* z        = a.logits + row * a.ldl;
-  const RowVecs<T> rv(z, a.vocab);
-  const int j0  = int(rank) * a.per_cta;
-  const int j1  = j0 + a.per_cta < rv.n ? j0 + a.per_cta : rv.n;
+  const RowPart<T> part(z, a.vocab, int(rank) * a.per_cta, a.per_cta);
   const float c = float(1.4426950408889634 / a.temperature);
   if (warp == NW) {  // the list
     if (kGrad || rank == 0) {
       for (int j = lane; j < k; j += 32) {
-        fetch_entry(a, row, j, &id[j], &logp[j]);
-        zid[j] = id[j] >= 0 ? FloatIo<T>::up(z[id[j]]) : 0.0f;
+        Entry entry;
+        entry.ask(a, row, j);
+        const int at = entry.id(a.vocab);
+        id[j]        = at;
+        zid[j]       = at >= 0 ? FloatIo<T>::up(z[at]) : 0.0f;
+        logp[j]      = entry.y;
       }
       const bool some = weigh_list(id, logp, k, float(1.0 / a.temperature));
       if (lane == 0) some_s = some;
@@ -532,22 +781,33 @@ distill_stream_kernel(const Args<T> a)
     cluster_wait();
   } else {
     float m = -INFINITY, s = 0.0f;  // as ExpSum
-    Vec cur[NV], nxt[NV];
-    auto fetch = [&](Vec(&v)[NV], int j) {
+    auto request = [&](int j, int stage) {  // vectors [j, j + NV * NT) of the part
+      Vec* to       = ring + stage * (NT * NV) + tid;
+      const T* from = part.at + (j + tid) * VE;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int q = j + i * NT + tid;
-        if (q < j1) v[i] = rv.load(z, q);
+      for (int i = 0; i < NV; ++i)
+        if (part.whole(j + i * NT + tid)) copy_async16(to + i * NT, from + i * (NT * VE));
+      if (part.edges() || j + NV * NT > part.n) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          const int q = j + i * NT + tid;
+          if (!part.whole(q)) to[i * NT] = q < part.n ? part.load_edge(q) : minus_inf<T>();
+        }
       }
+      copy_commit();
     };
-    auto use = [&](const Vec(&v)[NV], int j) {
+    const Pair mul = pair(c, c);
+    auto use = [&](const Vec* slot, int j) {
+      Pair e[NV * VE / 2];
       float top = m;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (j + i * NT + tid < j1) {
+        const Vec v = slot[i * NT + tid];  // -inf behind the end of the part
 #pragma unroll
-          for (int q = 0; q < VE; ++q)
-            top = fmaxf(top, FloatIo<T>::up(v[i].e[q]));
+        for (int q = 0; q < VE / 2; ++q) {
+          e[i * VE / 2 + q] = up2<T>(v, q);
+          const float2 f    = split(e[i * VE / 2 + q]);
+          top               = max3(top, f.x, f.y);
         }
       }
       if (top > m) {
@@ -555,22 +815,33 @@ distill_stream_kernel(const Args<T> a)
         m = top;
       }
       const float base = m == -INFINITY ? 0.0f : m;
+      const Pair sub   = pair(-base, -base);
+      Pair sum0 = pair(s, 0.0f), sum1 = pair(0.0f, 0.0f);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (j + i * NT + tid < j1) {
+        if (j + i * NT + warp * 32 < part.n) {
 #pragma unroll
-          for (int q = 0; q < VE; ++q)
-            s += ex2((FloatIo<T>::up(v[i].e[q]) - base) * c);
+          for (int q = i * VE / 2; q < (i + 1) * VE / 2; q += 2) {
+            sum0 = add2(sum0, ex2_2(mul2(add2(e[q], sub), mul)));
+            sum1 = add2(sum1, ex2_2(mul2(add2(e[q + 1], sub), mul)));
+          }
         }
       }
+      const float2 s2 = split(add2(sum0, sum1));
+      s               = s2.x + s2.y;
     };
-    fetch(cur, j0);
-    for (int j = j0; j < j1; j += 2 * NV * NT) {
-      fetch(nxt, j + NV * NT);
-      use(cur, j);
-      fetch(cur, j + 2 * NV * NT);
-      use(nxt, j + NV * NT);
+    constexpr int kChunk = NV * NT;
+#pragma unroll
+    for (int d = 0; d < kStreamDepth - 1; ++d)
+      request(d * kChunk, d);
+    int stage = 0;
+    for (int j = 0; j < part.n; j += kChunk) {
+      copy_wait<kStreamDepth - 2>();
+      use(ring + stage * kChunk, j);
+      request(j + (kStreamDepth - 1) * kChunk, stage == 0 ? kStreamDepth - 1 : stage - 1);
+      stage = stage + 1 == kStreamDepth ? 0 : stage + 1;
     }
+    copy_wait<0>();
     const ExpSum w = warp_join({m, s}, c);
     cluster_wait();
     if (lane < int(size)) cluster_store(&parts[rank * NW + warp], unsigned(lane), make_float2(w.m, w.s));
@@ -598,22 +869,23 @@ distill_stream_kernel(const Args<T> a)
     const float l2s    = log2f(all.s);
     const auto q       = [&](float x) { return ex2((x - all.m) * c - l2s); };
     T* g               = a.grad + row * a.ldg;
-    const bool same    = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
-    for (int j = j0 + tid; j < j1 && warp < NW; j += NT) {
-      const Vec v = rv.load(z, j);
+    const bool same    = same_phase(g, z);
+    for (int j = tid; j < part.n && warp < NW; j += NT) {
+      const Vec v = part.load(j);
       Vec o;
 #pragma unroll
-      for (int e = 0; e < VE; ++e)
-        o.e[e] = FloatIo<T>::down(some ? q(FloatIo<T>::up(v.e[e])) * factor : 0.0f);
-      rv.store(g, j, o, same);
+      for (int e = 0; e < VE / 2; ++e) {
+        const float2 f = up_pair<T>(v, e);
+        down_pair<T>(o, e, some ? make_float2(q(f.x) * factor, q(f.y) * factor) : make_float2(0.0f, 0.0f));
+      }
+      part.store(g + part.first, j, o, same);
     }
     __syncthreads();
-    const int lo = rv.first(j0) > 0 ? rv.first(j0) : 0;
-    const int hi = rv.first(j1) < a.vocab ? rv.first(j1) : a.vocab;
     for (int j = tid; j < k && some; j += NT + 32) {
       const int t = id[j];
       float w;
-      if (t >= lo && t < hi && listed_weight(id, logp, k, j, &w)) g[t] = FloatIo<T>::down(factor * (q(zid[j]) - w));
+      if (t >= part.token0 && t < part.token1 && listed_weight(id, logp, k, j, &w))
+        g[t] = FloatIo<T>::down(factor * (q(zid[j]) - w));
     }
   }
 }
@@ -635,15 +907,10 @@ distill_grad_kernel(const Args<T> a, unsigned parts)
   float* zid  = logp + k;
   grid_dep_sync();
   const int64_t row = int64_t(blockIdx.x) / parts;
-  const int part    = int(int64_t(blockIdx.x) - row * parts);
   const T* z        = a.logits + row * a.ldl;
-  const RowVecs<T> rv(z, a.vocab);
-  const int j0  = part * (NT * NV);
-  const int j1  = j0 + NT * NV < rv.n ? j0 + NT * NV : rv.n;
+  const RowPart<T> part(z, a.vocab, int(int64_t(blockIdx.x) - row * parts) * (NT * NV), NT * NV);
   const int tid = int(threadIdx.x);
-  if (j0 >= j1) return;  // uniform over the CTA
-  const int lo = rv.first(j0) > 0 ? rv.first(j0) : 0;
-  const int hi = rv.first(j1) < a.vocab ? rv.first(j1) : a.vocab;
+  if (part.n <= 0) return;  // uniform over the CTA
   // 1 / T in two fp32 pieces: rounded to one it would scale the row by its largest logit's share of the error
   // (-inf is taken as the lowest finite value: -inf times a zero piece would be NaN)
   const double inv = 1.0 / a.temperature;
@@ -653,17 +920,21 @@ distill_grad_kernel(const Args<T> a, unsigned parts)
     const float f = fmaxf(x, -FLT_MAX);
     return ex2(fmaf(f, lo_t, fmaf(f, hi_t, -lse)) * 1.4426950408889634f);
   };
-  VecOf<T, VE> raw[NV];
+  Words4 raw[NV];
   if (tid < NT) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = j0 + i * NT + tid;
-      if (j < j1) raw[i] = rv.load(z, j);
+      const int j = i * NT + tid;
+      if (j < part.n) raw[i] = part.load(j);
     }
   } else {
     for (int j = tid - NT; j < k; j += 32) {
-      fetch_entry(a, row, j, &id[j], &logp[j]);
-      zid[j] = id[j] >= lo && id[j] < hi ? FloatIo<T>::up(z[id[j]]) : 0.0f;
+      Entry entry;
+      entry.ask(a, row, j);
+      const int at = entry.id(a.vocab);
+      id[j]        = at;
+      zid[j]       = at >= part.token0 && at < part.token1 ? FloatIo<T>::up(z[at]) : 0.0f;
+      logp[j]      = entry.y;
     }
     const bool some = weigh_list(id, logp, k, float(1.0 / a.temperature));
     if (tid == NT) some_s = some;
@@ -672,17 +943,19 @@ distill_grad_kernel(const Args<T> a, unsigned parts)
   const bool some    = some_s != 0;
   const float factor = some ? float(double(a.grad_loss[row]) * a.temperature) : 0.0f;
   T* g               = a.grad + row * a.ldg;
-  const bool same    = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
+  const bool same    = same_phase(g, z);
   if (tid < NT) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = j0 + i * NT + tid;
-      if (j < j1) {
-        VecOf<T, VE> o;
+      const int j = i * NT + tid;
+      if (j < part.n) {
+        Words4 o;
 #pragma unroll
-        for (int e = 0; e < VE; ++e)
-          o.e[e] = FloatIo<T>::down(some ? q(FloatIo<T>::up(raw[i].e[e])) * factor : 0.0f);
-        rv.store(g, j, o, same);
+        for (int e = 0; e < VE / 2; ++e) {
+          const float2 f = up_pair<T>(raw[i], e);
+          down_pair<T>(o, e, some ? make_float2(q(f.x) * factor, q(f.y) * factor) : make_float2(0.0f, 0.0f));
+        }
+        part.store(g + part.first, j, o, same);
       }
     }
   }
@@ -690,7 +963,8 @@ distill_grad_kernel(const Args<T> a, unsigned parts)
   for (int j = tid; j < k && some; j += NT + 32) {
     const int t = id[j];
     float w;
-    if (t >= lo && t < hi && listed_weight(id, logp, k, j, &w)) g[t] = FloatIo<T>::down(factor * (q(zid[j]) - w));
+    if (t >= part.token0 && t < part.token1 && listed_weight(id, logp, k, j, &w))
+        g[t] = FloatIo<T>::down(factor * (q(zid[j]) - w));
   }
 }
 
@@ -781,59 +1055,68 @@ inline int64_t resident_clusters(Kernel kern, int size, int threads, size_t smem
   return have.n;
 }
 
-template <typename T, int NT>
-inline cudaError_t launch_step(Args<T> a, int64_t most, int size, cudaStream_t stream)
+template <typename T, int NT, bool kEven>
+inline cudaError_t launch_step_as(Args<T> a, int64_t most, int size, cudaStream_t stream)
 {
-  auto kern         = distill_step_kernel<T, NT>;
-  const size_t smem = size_t(kStages) * NT * kStepNv * 16 + size_t(a.list.k) * 32;
+  auto kern         = distill_step_kernel<T, NT, kEven>;
+  const size_t smem = size_t(kStages) * NT * kStepNv * 16 + size_t(a.list.k) * 36;
   a.per_cta         = int(ceil_div<int64_t>(most, size));
   cudaError_t e     = ensure_dynamic_smem(kern, smem);
   if (e != cudaSuccess) return e;
-  const int64_t fit      = resident_clusters(kern, size, NT, smem);
+  const int64_t fit      = resident_clusters(kern, size, NT + 64, smem);
   const int64_t clusters = a.n_rows < fit ? a.n_rows : fit;
-  return launch_clusters(kern, a, clusters * size, size, NT, smem, stream);
+  return launch_clusters(kern, a, clusters * size, size, NT + 64, smem, stream);
+}
+
+template <typename T, int NT>
+inline cudaError_t launch_step(const Args<T>& a, int64_t most, int size, cudaStream_t stream)
+{
+  const bool even = a.n_rows == 1 || uintptr_t(a.ldl) * sizeof(T) % 16 == 0;
+  return even ? launch_step_as<T, NT, true>(a, most, size, stream) : launch_step_as<T, NT, false>(a, most, size, stream);
 }
 
 template <typename T, int NT, bool kGrad>
 inline cudaError_t launch_stream(Args<T> a, int64_t most, int size, cudaStream_t stream)
 {
   a.per_cta              = int(ceil_div<int64_t>(most, size));
-  const size_t smem      = size_t(a.list.k) * 12;
+  const size_t smem      = size_t(kStreamDepth) * NT * kStreamNv * 16 + size_t(a.list.k) * 12;
   const int64_t max_rows = int64_t(0x7fffffff) / size;
+  cudaError_t e          = ensure_dynamic_smem(distill_stream_kernel<T, NT, kGrad>, smem);
+  if (e != cudaSuccess) return e;
   for (int64_t r0 = 0; r0 < a.n_rows; r0 += max_rows) {
-    const int64_t n     = a.n_rows - r0 < max_rows ? a.n_rows - r0 : max_rows;
-    const cudaError_t e = launch_clusters(distill_stream_kernel<T, NT, kGrad>, rows_from(a, r0, n), n * size, size,
+    const int64_t n = a.n_rows - r0 < max_rows ? a.n_rows - r0 : max_rows;
+    e = launch_clusters(distill_stream_kernel<T, NT, kGrad>, rows_from(a, r0, n), n * size, size,
                                           NT + 32, smem, stream);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 
-// Loss and gradient: a row is held by the CTAs of a cluster, NT x kStepNv vectors each; small vocabularies take small
-// CTAs, and a row of more than 8 CTAs of 1024 threads is read twice.
+// Loss and gradient: a row is held by the CTAs of a cluster, 4096 vectors (64 KB) each; small vocabularies take small
+// CTAs, and a row of more than 8 full ones is read twice, as are rows whose list does not fit beside the buffers.
 template <typename T>
 inline cudaError_t launch_loss_and_grad(const Args<T>& a, cudaStream_t stream)
 {
   const int64_t most = most_vectors(a);
-  // (beside 192 KB of buffers a CTA of 1024 threads has room for lists of 960 entries)
-  if (a.list.k > 960) return launch_stream<T, 512, true>(a, most, 8, stream);
-  if (most <= 128 * kStepNv) return launch_step<T, 128>(a, most, 1, stream);
-  if (most <= 512 * kStepNv) return launch_step<T, 512>(a, most, 1, stream);
+  if (a.list.k > 900) return launch_stream<T, 256, true>(a, most, 8, stream);
+  if (most <= 64 * kStepNv) return launch_step<T, 64>(a, most, 1, stream);
+  if (most <= 256 * kStepNv) return launch_step<T, 256>(a, most, 1, stream);
   for (int size = 1; size <= 8; size *= 2)
-    if (most <= int64_t(1024) * kStepNv * size) return launch_step<T, 1024>(a, most, size, stream);
-  return launch_stream<T, 512, true>(a, most, 8, stream);
+    if (most <= int64_t(512) * kStepNv * size) return launch_step<T, 512>(a, most, size, stream);
+  return launch_stream<T, 256, true>(a, most, 8, stream);
 }
 
-// Loss: CTAs of 128 threads for short rows; rows are split over up to 8 CTAs while there are fewer than two per SM.
+// Loss: rows are split over up to 8 CTAs, of at least two chunks each, while there are fewer than sixteen CTAs per SM
+// (2048 x 131072: the last CTAs of two per SM would leave most of the machine idle for a tenth of the time).
 template <typename T>
 inline cudaError_t launch_loss(const Args<T>& a, cudaStream_t stream)
 {
   const int64_t most = most_vectors(a);
-  if (most <= 128 * kStreamNv * 2) return launch_stream<T, 128, false>(a, most, 1, stream);
+  if (most <= 128 * kStreamNv) return launch_stream<T, 128, false>(a, most, 1, stream);
   int size = 1;
-  while (size < 8 && a.n_rows * size < 2 * int64_t(sm_count()) && most >= int64_t(512) * kStreamNv * size)
+  while (size < 8 && a.n_rows * size < 16 * int64_t(sm_count()) && most >= int64_t(256) * kStreamNv * 4 * size)
     size *= 2;
-  return launch_stream<T, 512, false>(a, most, size, stream);
+  return launch_stream<T, 256, false>(a, most, size, stream);
 }
 
 template <typename T>

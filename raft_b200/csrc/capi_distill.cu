@@ -39,6 +39,7 @@ static detail::distill::Args<T> distill_args(const void* logits, int64_t ldl, vo
   a.n_rows      = n_rows;
   a.vocab       = int(vocab);
   a.temperature = temperature;
+  a.ctl         = detail::ring_ctl(kernel_status_word());
   return a;
 }
 

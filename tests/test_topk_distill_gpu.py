@@ -390,3 +390,26 @@ def test_refusals(cuda):
         linalg.topk_distill_step(big[:4], ids, teacher, weight, grad=big[1:])
     with pytest.raises(ValueError):
         linalg.topk_distill_grad(logits, ids, teacher, lse[:2], weight)
+
+
+def test_a_record_that_never_arrives_ends_in_nan_and_a_status(cuda, knobs):
+    """The exchange between the CTAs of a row waits with a limit: the first CTA's record for the third row of its
+    cluster is withheld, so that its cluster gives up on that row, its later rows are NaN, and all others are right."""
+    logits, ids, teacher, weight = make(300, 70000, 8, torch.bfloat16, cuda)
+    exp = linalg.topk_distill_step(logits, ids, teacher, weight)
+    assert linalg.last_kernel_status(cuda) == _lib.OK
+    linalg.set_wait_limit_ms(50)
+    knobs(B2R_TEST_SKIP_TILE=3)
+    try:
+        loss, lse, grad = linalg.topk_distill_step(logits, ids, teacher, weight)
+        assert linalg.last_kernel_status(cuda) == _lib.ERR_TIMEOUT
+    finally:
+        knobs(B2R_TEST_SKIP_TILE=None)
+        linalg.set_wait_limit_ms(0)
+    bad = torch.isnan(grad).any(1)
+    assert 0 < int(bad.sum()) < 150
+    assert torch.equal(grad[~bad], exp[2][~bad])
+    again = linalg.topk_distill_step(logits, ids, teacher, weight)
+    assert linalg.last_kernel_status(cuda) == _lib.OK
+    for a, b in zip(again, exp):
+        assert torch.equal(a, b)
