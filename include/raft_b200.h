@@ -358,6 +358,44 @@ B2R_API int b2r_topk_distill_grad(void* grad,
                                   b2r_stream_t stream);
 
 /*
+ * One token for every row of `logits` [n_rows x vocab] from a uniform number u in [0, 1) given for the row. With z the
+ * row, zmax its largest element, T the temperature and w_v = exp((z_v - zmax) / T), tokens in the order of falling
+ * logits (equal ones by rising token):
+ *   kept  the first top_k of the order (top_k <= 0: all); of those the tokens with w >= min_p (at most 1); of those
+ *         the shortest beginning of the order whose weight is at least top_p of their whole weight (top_p >= 1: all;
+ *         always at least one token);
+ *   drawn the first kept token, by token number, at which the running sum of w exceeds u * (sum of the kept w).
+ * T <= 0 (or NaN) takes the largest logit, the lowest token of equals. NaN logits count as -inf; weights relative to a
+ * +inf logit are 0, its own 1. A row of -inf alone has no token: -1. Weights are fp64, their sums exact integers, so a
+ * row's token does not depend on the other rows, the split over CTAs or the run.
+ * tokens (B2R_I32 or B2R_I64, out_dtype) and logprobs (fp32, may be NULL: log of the probability with which the token
+ * was drawn; 0 for T <= 0, -inf for no token) have n_rows elements. Parameters are fp32 / int32 device vectors of
+ * n_rows elements, or NULL for the value given for all rows.
+ */
+typedef struct {
+  int32_t dtype;     /* of the logits: B2R_F32, B2R_F16 or B2R_BF16 */
+  int32_t out_dtype; /* of the tokens: B2R_I32 or B2R_I64           */
+  int64_t n_rows;
+  int64_t vocab;
+  int64_t ld; /* row stride of the logits, in elements */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int32_t top_k_all;
+  float top_p_all;
+  float min_p_all;
+} b2r_sample_desc;
+
+B2R_API int b2r_sample_tokens(const b2r_sample_desc* desc,
+                              void* tokens,
+                              float* logprobs,
+                              const void* logits,
+                              const float* uniform,
+                              b2r_stream_t stream);
+
+/*
  * Column sums of a row-major fp32 matrix without any allocation:
  *     out[j] = final_op(sum over i of in[i][j]),   in [n_rows x n_cols], out [n_cols]
  * This entry point has no counterpart in the reference. It is b2r_reduce's column path

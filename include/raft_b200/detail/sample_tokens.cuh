@@ -1,0 +1,546 @@
+// One token per row of logits by temperature, top-k, top-p and min-p, from a given uniform number.
+//
+// With z the row's logits, zmax the largest, T the temperature and w_v = exp((z_v - zmax) / T), tokens are ordered by
+// falling logit, equal logits by rising token. Kept are the first top_k of that order, of those the tokens with
+// w >= min_p, and of those the shortest beginning of the order whose weight reaches top_p of their whole weight. Drawn
+// is the first kept token, BY TOKEN, at which the running weight exceeds u times the kept weight. T <= 0 takes the
+// largest logit (the lowest token of equals). NaN logits count as -inf; a row of nothing else has no token: -1.
+//
+// Which side of a border a token falls on is decided by sums over the vocabulary in which a token may weigh 1e-6 of
+// the whole, so weights are computed in fp64 and summed as INTEGERS of 2^-shift, shift = 62 - ceil(log2 vocab) (45 bits
+// for 131072 tokens): exact, the same whatever the order, the split of the row or the number of rows of the call.
+//
+// A cluster of CTAs takes a row, every CTA a part, which it keeps in shared memory. Thresholds in the order are found
+// by radix selection on the logits' bits, made to rise with their value: histograms of counts (top-k) or of weights
+// (top-p), summed over the cluster through distributed shared memory, a digit at a time.
+#pragma once
+
+#include "launch.cuh"
+#include "topk_distill.cuh"  // RowPart, cluster primitives
+
+namespace raft_b200 {
+namespace detail {
+namespace sample {
+
+using distill::RowPart;
+using u64 = unsigned long long;
+
+constexpr int kThreads    = 512;
+constexpr int kWarps      = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int kDigitBits  = 11;
+constexpr int kBins       = 1 << kDigitBits;
+constexpr int kMaxPartKb  = 160;  // of a row in a CTA's shared memory
+
+template <typename T>
+struct Args {
+  const T* logits;
+  int64_t ldl;
+  const float* uniform;
+  const float* temperature;  // each may be null: the value for all rows counts then
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all;
+  int top_k_all;
+  float top_p_all, min_p_all;
+  void* out;
+  int out64;
+  float* logprobs;  // may be null
+  int64_t n_rows;
+  int vocab;
+  int per_cta;  // vectors of a row per CTA
+  int shift;    // weights are integers of 2^-shift
+};
+
+// The bits of an element as a number that rises with its value: -0 as +0, NaN as -inf.
+template <typename T>
+struct Key;
+template <>
+struct Key<float> {
+  static constexpr int kBits        = 32;
+  static constexpr unsigned kNegInf = 0x007fffffu;
+  B2R_DI static unsigned of(const Words4& v, int e)
+  {
+    const unsigned b = v.w[e];
+    if ((b & 0x7fffffffu) > 0x7f800000u) return kNegInf;
+    return (b & 0x80000000u) ? (b == 0x80000000u ? 0x80000000u : ~b) : (b | 0x80000000u);
+  }
+  B2R_DI static float value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+  // lowest key whose value is at least x
+  B2R_DI static unsigned at_least(double x)
+  {
+    const float f = __double2float_ru(x);
+    Words4 v;
+    v.w[0] = __float_as_uint(f);
+    return of(v, 0);
+  }
+};
+template <typename T, unsigned Inf>
+struct Key16 {
+  static constexpr int kBits        = 16;
+  static constexpr unsigned kNegInf = 0x7fffu - Inf;  // ~(0x8000 | Inf) in 16 bits
+  B2R_DI static unsigned of_bits(unsigned b)
+  {
+    if ((b & 0x7fffu) > Inf) return kNegInf;
+    return (b & 0x8000u) ? (b == 0x8000u ? 0x8000u : (~b & 0xffffu)) : (b | 0x8000u);
+  }
+  B2R_DI static unsigned of(const Words4& v, int e) { return of_bits((e & 1) ? v.w[e / 2] >> 16 : v.w[e / 2] & 0xffffu); }
+  B2R_DI static float value(unsigned k)
+  {
+    const uint16_t b = uint16_t((k & 0x8000u) ? (k & 0x7fffu) : ~k);
+    T x;
+    memcpy(&x, &b, 2);
+    return FloatIo<T>::up(x);
+  }
+  // lowest key whose value is at least x: by bisection of the keys, whose values rise
+  B2R_DI static unsigned at_least(double x)
+  {
+    unsigned lo = kNegInf, hi = 0x8000u + Inf;  // -inf ... +inf
+    while (lo < hi) {
+      const unsigned mid = (lo + hi) >> 1;
+      if (double(value(mid)) >= x)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    return lo;
+  }
+};
+template <>
+struct Key<__half> : Key16<__half, 0x7c00u> {};
+template <>
+struct Key<__nv_bfloat16> : Key16<__nv_bfloat16, 0x7f80u> {};
+
+B2R_DI u64 warp_sum_u64(u64 v)
+{
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    v += __shfl_xor_sync(distill::kFull, v, o);
+  return v;
+}
+B2R_DI u64 warp_scan_u64(u64 v)  // inclusive
+{
+  const int lane = int(threadIdx.x) & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(distill::kFull, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+B2R_DI void cluster_store_u64(u64* p, unsigned rank, u64 v)
+{
+  const unsigned local = smem_u32(p);
+  unsigned remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote), "l"(v) : "memory");
+}
+B2R_DI unsigned cluster_load_u32(const unsigned* p, unsigned rank)
+{
+  const unsigned local = smem_u32(p);
+  unsigned remote, v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  return v;
+}
+B2R_DI void cluster_sync()
+{
+  distill::cluster_arrive();
+  distill::cluster_wait();
+}
+
+template <typename T, bool kCached>
+__global__ void __launch_bounds__(kThreads)
+sample_kernel(const Args<T> a)
+{
+  constexpr int VE = Vec16Of<T>::value;
+  using K          = Key<T>;
+  extern __shared__ __align__(16) unsigned char sample_smem[];
+  __shared__ unsigned hist[2][kBins];           // low and high words of the bins' sums
+  __shared__ u64 bins[kBins];                   // sums over the cluster of the bins this CTA looks after
+  __shared__ u64 posted[4][kMaxCluster];        // a value from every CTA of the cluster, four exchanges deep
+  __shared__ u64 result[2][2];
+  __shared__ u64 warp_part[kWarps];
+  __shared__ u64 carry;
+  Words4* slice = reinterpret_cast<Words4*>(sample_smem);  // [per_cta] if kCached
+  u64* units    = reinterpret_cast<u64*>(slice + (kCached ? a.per_cta : 0));  // sums of 32 vectors each, in order
+  const unsigned rank = distill::cluster_rank();
+  const unsigned size = distill::cluster_size();
+  const int tid = int(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+  distill::cluster_arrive();
+  grid_dep_sync();
+
+  const int64_t row = int64_t(blockIdx.x) / size;
+  const T* z        = a.logits + row * a.ldl;
+  const RowPart<T> part(z, a.vocab, int(rank) * a.per_cta, a.per_cta);
+  const float temp   = a.temperature != nullptr ? a.temperature[row] : a.temperature_all;
+  const int top_k    = a.top_k != nullptr ? a.top_k[row] : a.top_k_all;
+  const float top_p  = a.top_p != nullptr ? a.top_p[row] : a.top_p_all;
+  const float min_p  = a.min_p != nullptr ? a.min_p[row] : a.min_p_all;
+  const float u      = a.uniform[row];
+  const bool greedy  = !(temp > 0.0f);
+  const auto vec     = [&](int j) { return kCached ? slice[j] : part.load(j); };
+  int exchanges      = 0;
+
+  // every CTA's v, known to all afterwards (four calls long)
+  auto post = [&](u64 v) {
+    u64* slot = posted[exchanges & 3];
+    ++exchanges;
+    if (tid < int(size)) cluster_store_u64(&slot[rank], unsigned(tid), v);
+    cluster_sync();
+    return slot;
+  };
+  auto block_sum = [&](u64 v) {  // to all threads
+    v = warp_sum_u64(v);
+    __syncthreads();
+    if (lane == 0) warp_part[warp] = v;
+    __syncthreads();
+    u64 s = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+      s += warp_part[w];
+    return s;
+  };
+
+  // the row, and its largest key
+  unsigned kmax = 0;
+  for (int j = tid; j < part.n; j += kThreads) {
+    const Words4 v = part.load(j);
+    if (kCached) slice[j] = v;
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+      kmax = max(kmax, K::of(v, e));
+  }
+  kmax = __reduce_max_sync(distill::kFull, kmax);
+  if (lane == 0) warp_part[warp] = kmax;
+  __syncthreads();
+  for (int w = 0; w < kWarps; ++w)
+    kmax = max(kmax, unsigned(warp_part[w]));
+  distill::cluster_wait();
+  {
+    const u64* all = post(kmax);
+    for (unsigned r = 0; r < size; ++r)
+      kmax = max(kmax, unsigned(all[r]));
+  }
+  auto write = [&](int64_t token, float logprob) {  // by one thread of the cluster
+    if (a.out64)
+      static_cast<long long*>(a.out)[row] = token;
+    else
+      static_cast<int*>(a.out)[row] = int(token);
+    if (a.logprobs != nullptr) a.logprobs[row] = logprob;
+  };
+  if (kmax <= K::kNegInf) {  // nothing to draw from
+    if (rank == 0 && tid == 0) write(-1, -INFINITY);
+    return;
+  }
+  const double zmax  = double(K::value(kmax));
+  const double slope = 1.4426950408889634 / double(temp);
+  const double unit  = double(u64(1) << a.shift);
+  const auto weight  = [&](unsigned key) -> u64 {
+    if (key == kmax) return u64(1) << a.shift;
+    const double x = (double(K::value(key)) - zmax) * slope;
+    return x <= 0.0 ? u64(__double2ull_rn(exp2(x) * unit)) : 0;  // (0 for -inf * 0: a +inf logit at infinite temperature)
+  };
+
+  // kept: key > tau, or key == tau and token <= last
+  unsigned tau = K::kNegInf + 1;
+  int last     = 0x7fffffff;
+  const auto kept = [&](unsigned key, int token) { return key > tau || (key == tau && token <= last); };
+
+  // Sums of value(key, token) over runs of 32 vectors; *before: of the CTAs ahead of this one. Returns the whole sum.
+  auto sum_in_order = [&](auto value, u64* before, u64* mine) {
+    u64 own = 0;
+    for (int j0 = warp * 32; j0 < part.n; j0 += kThreads) {
+      u64 s = 0;
+      if (j0 + lane < part.n) {
+        const Words4 v = vec(j0 + lane);
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          s += value(K::of(v, e), part.first + (j0 + lane) * VE + e);
+      }
+      s = warp_sum_u64(s);
+      if (lane == 0) units[j0 / 32] = s;
+      own += s;
+    }
+    __syncthreads();
+    if (lane == 0) warp_part[warp] = own;
+    __syncthreads();
+    own = 0;
+    for (int w = 0; w < kWarps; ++w)
+      own += warp_part[w];
+    const u64* all = post(own);
+    u64 total = 0, ahead = 0;
+    for (unsigned r = 0; r < size; ++r) {
+      total += all[r];
+      ahead += r < rank ? all[r] : 0;
+    }
+    *before = ahead;
+    *mine   = own;
+    return total;
+  };
+  // by warp 0 of the CTA whose range holds `target` (relative to the CTA's own beginning): the token at which the
+  // running sum exceeds it, and that token's key
+  auto locate = [&](auto value, u64 target, unsigned* key) {
+    const int n_units = (part.n + 31) / 32;
+    u64 run = 0;
+    int at  = 0;
+    for (int b = 0; b < n_units; b += 32) {
+      const u64 s    = b + lane < n_units ? units[b + lane] : 0;
+      const u64 incl = run + warp_scan_u64(s);
+      const unsigned over = __ballot_sync(distill::kFull, incl > target);
+      if (over != 0u) {
+        const int l = __ffs(int(over)) - 1;
+        at          = b + l;
+        run         = __shfl_sync(distill::kFull, incl - s, l);
+        break;
+      }
+      run = __shfl_sync(distill::kFull, incl, 31);
+    }
+    const int j = at * 32 + lane;
+    Words4 v    = distill::minus_inf<T>();
+    u64 s       = 0;
+    if (j < part.n) {
+      v = vec(j);
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        s += value(K::of(v, e), part.first + j * VE + e);
+    }
+    const u64 incl      = run + warp_scan_u64(s);
+    const unsigned over = __ballot_sync(distill::kFull, incl > target);
+    const int l         = __ffs(int(over)) - 1;
+    u64 upto            = incl - s;
+    int token           = -1;
+    unsigned found      = 0;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const int t = part.first + j * VE + e;
+      upto += value(K::of(v, e), t);
+      if (token < 0 && upto > target) {
+        token = t;
+        found = K::of(v, e);
+      }
+    }
+    *key = __shfl_sync(distill::kFull, found, l);
+    return __shfl_sync(distill::kFull, token, l);
+  };
+  // The border of the order at which the sum of value(key) over the kept tokens reaches `target` (at least 1, at most
+  // the whole sum): its key in *border, the sum over larger keys in *above. With kCount the values are 1.
+  // A target above the whole sum, which is returned in *total: the border is below every kept key, false.
+  auto select = [&](auto count, auto value, auto target_of, unsigned* border, u64* above, u64* total) {
+    constexpr bool kCount = decltype(count)::value;
+    unsigned prefix = 0;  // bits of the border found so far
+    int left        = K::kBits;
+    u64 over        = 0;
+    u64 target      = 0;
+    while (left > 0) {
+      const int bits  = left > kDigitBits ? kDigitBits : left;
+      const int shift = left - bits;
+      const int n     = 1 << bits;
+      for (int i = tid; i < n; i += kThreads)
+        hist[0][i] = hist[1][i] = 0;
+      __syncthreads();
+      for (int j = tid; j < part.n; j += kThreads) {
+        const Words4 v = vec(j);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const unsigned key = K::of(v, e);
+          if ((left == K::kBits || (key >> left) == prefix) && kept(key, part.first + j * VE + e)) {
+            const unsigned d = (key >> shift) & unsigned(n - 1);
+            if constexpr (kCount) {
+              atomicAdd(&hist[0][d], 1u);
+            } else {
+              const u64 w = value(key);
+              if (w != 0) {  // a 64-bit sum by its words: the low one tells when it wraps
+                const unsigned lo   = unsigned(w);
+                const unsigned old  = atomicAdd(&hist[0][d], lo);
+                const unsigned high = unsigned(w >> 32) + (old + lo < old ? 1u : 0u);
+                if (high != 0u) atomicAdd(&hist[1][d], high);
+              }
+            }
+          }
+        }
+      }
+      // this CTA's share of the bins, over the cluster; bins fall with the rank, as the order does
+      cluster_sync();
+      const int own_bins = n / int(size);
+      const int top      = n - 1 - int(rank) * own_bins;  // its largest
+      u64 mine           = 0;
+      for (int i = tid; i < own_bins; i += kThreads) {
+        u64 s = 0;
+        for (unsigned r = 0; r < size; ++r) {
+          s += cluster_load_u32(&hist[0][top - i], r);
+          if (!kCount) s += u64(cluster_load_u32(&hist[1][top - i], r)) << 32;
+        }
+        bins[i] = s;
+        mine += s;
+      }
+      mine           = block_sum(mine);
+      const u64* all = post(mine);
+      u64 whole = 0, ahead = over;
+      for (unsigned r = 0; r < size; ++r) {
+        whole += all[r];
+        ahead += r < rank ? all[r] : 0;
+      }
+      if (left == K::kBits) {
+        *total = whole;
+        target = target_of(whole);
+        if (target > whole) return false;
+      }
+      u64* res = result[(K::kBits - left) / kDigitBits & 1];
+      if (ahead < target && target <= ahead + mine && warp == 0) {  // the border is in one of this CTA's bins
+        u64 run = ahead;
+        for (int b = 0; b < own_bins; b += 32) {
+          const u64 s         = b + lane < own_bins ? bins[b + lane] : 0;
+          const u64 incl      = run + warp_scan_u64(s);
+          const unsigned full = __ballot_sync(distill::kFull, incl >= target);
+          if (full != 0u) {
+            const int l       = __ffs(int(full)) - 1;
+            const u64 before  = __shfl_sync(distill::kFull, incl - s, l);
+            const unsigned bin = unsigned(top - b - l);
+            if (lane < int(size)) {
+              cluster_store_u64(&res[0], unsigned(lane), bin);
+              cluster_store_u64(&res[1], unsigned(lane), before);
+            }
+            break;
+          }
+          run = __shfl_sync(distill::kFull, incl, 31);
+        }
+      }
+      cluster_sync();
+      prefix = (prefix << bits) | unsigned(res[0]);
+      over   = res[1];
+      left   = shift;
+    }
+    *border = prefix;
+    *above  = over;
+    return true;
+  };
+  // the token of the `nth` (from 1) kept element whose key is tau, as a limit for all CTAs
+  auto limit_ties = [&](u64 nth) {
+    const auto is_tie = [&](unsigned key, int token) -> u64 { return key == tau && token <= last ? 1 : 0; };
+    u64 before, mine;
+    const u64 total = sum_in_order(is_tie, &before, &mine);
+    if (nth >= total) return;  // all of them
+    u64 found = 0;
+    if (before < nth && nth <= before + mine) {
+      if (warp == 0) {
+        unsigned key;
+        found = u64(locate(is_tie, nth - 1 - before, &key)) + 1;
+        if (lane == 0) carry = found;
+      }
+      __syncthreads();
+      found = carry;
+    }
+    const u64* all = post(found);
+    for (unsigned r = 0; r < size; ++r)
+      if (all[r] != 0) last = int(all[r]) - 1;
+  };
+
+  if (greedy) {
+    tau = kmax;
+    const auto is_max = [&](unsigned key, int) -> u64 { return key == kmax ? 1 : 0; };
+    u64 before, mine;
+    (void)sum_in_order(is_max, &before, &mine);
+    if (before == 0 && mine > 0 && warp == 0) {
+      unsigned key;
+      const int token = locate(is_max, 0, &key);
+      if (lane == 0) write(token, 0.0f);
+    }
+    return;
+  }
+  if (top_k > 0 && top_k < a.vocab) {
+    unsigned border;
+    u64 above, total;
+    if (select(std::true_type{}, weight, [&](u64) { return u64(top_k); }, &border, &above, &total)) {
+      tau = border;
+      limit_ties(u64(top_k) - above);
+    }
+  }
+  if (min_p > 0.0f) {
+    // w >= min_p, as a bound on the logit
+    const double p     = min_p < 1.0f ? double(min_p) : 1.0;
+    const unsigned low = p == 1.0 ? kmax : K::at_least(zmax + log2(p) / slope);
+    if (low > tau) {
+      tau  = low < kmax ? low : kmax;
+      last = 0x7fffffff;
+    }
+  }
+  if (top_p < 1.0f) {
+    unsigned border;
+    u64 above, total, target = 1;
+    const auto target_of = [&](u64 whole) {
+      const double t = ceil(double(top_p) * double(whole));
+      target         = t >= 1.0 ? u64(t) : 1;
+      if (target > whole) target = whole;
+      return target;
+    };
+    if (select(std::false_type{}, weight, target_of, &border, &above, &total)) {
+      const bool same = border == tau;
+      const u64 w     = weight(border);
+      tau             = border;
+      if (!same) last = 0x7fffffff;
+      limit_ties((target - above + w - 1) / w);
+    }
+  }
+  const auto kept_weight = [&](unsigned key, int token) -> u64 { return kept(key, token) ? weight(key) : 0; };
+  u64 before, mine;
+  const u64 total = sum_in_order(kept_weight, &before, &mine);
+  const double t  = double(u) * double(total);
+  u64 target      = t > 0.0 ? u64(t) : 0;
+  if (target >= total) target = total - 1;  // u of 1 (or more) takes the last kept token
+  if (before <= target && target < before + mine && warp == 0) {
+    unsigned key;
+    const int token = locate(kept_weight, target - before, &key);
+    if (lane == 0) write(token, float(log(double(weight(key)) / double(total))));
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side. The smallest cluster whose parts take at most 64 KB (three CTAs per SM), larger ones while there are
+// fewer than two CTAs per SM; parts of up to kMaxPartKb where eight CTAs are not enough, and beyond that rows are read
+// from memory in every pass.
+// ---------------------------------------------------------------------------------------
+template <typename T>
+inline cudaError_t launch_sample(Args<T> a, cudaStream_t stream)
+{
+  constexpr int VE   = Vec16Of<T>::value;
+  const int align    = common_alignment({reinterpret_cast<uintptr_t>(a.logits),
+                                         a.n_rows > 1 ? uintptr_t(a.ldl) * sizeof(T) : uintptr_t(0)});
+  const int64_t most = ceil_div<int64_t>((align >= 16 ? 0 : VE - 1) + int64_t(a.vocab), VE);
+  int size           = 1;
+  while (size < kMaxCluster && (most > int64_t(size) * 4096 ||
+                                (a.n_rows * size < 2 * int64_t(sm_count()) && most > int64_t(size) * 512)))
+    size *= 2;
+  a.per_cta         = int(ceil_div<int64_t>(most > 0 ? most : 1, size));
+  a.shift           = 62;
+  while (a.shift > 0 && (int64_t(1) << (62 - a.shift)) < a.vocab)
+    --a.shift;
+  const bool cached  = int64_t(a.per_cta) * 16 <= int64_t(kMaxPartKb) * 1024;
+  const size_t units = size_t(ceil_div(a.per_cta, 32)) * sizeof(u64);
+  const size_t smem  = (cached ? size_t(a.per_cta) * 16 : 0) + units;
+  const int64_t max_rows = int64_t(0x7fffffff) / size;
+  auto kern              = cached ? sample_kernel<T, true> : sample_kernel<T, false>;
+  cudaError_t e          = ensure_dynamic_smem(kern, smem);
+  if (e != cudaSuccess) return e;
+  for (int64_t r0 = 0; r0 < a.n_rows; r0 += max_rows) {
+    const int64_t n = a.n_rows - r0 < max_rows ? a.n_rows - r0 : max_rows;
+    Args<T> b       = a;
+    b.n_rows        = n;
+    b.logits += r0 * a.ldl;
+    b.uniform += r0;
+    if (b.temperature) b.temperature += r0;
+    if (b.top_k) b.top_k += r0;
+    if (b.top_p) b.top_p += r0;
+    if (b.min_p) b.min_p += r0;
+    if (b.logprobs) b.logprobs += r0;
+    b.out = static_cast<char*>(a.out) + r0 * (a.out64 ? 8 : 4);
+    e     = distill::launch_clusters(kern, b, n * size, size, kThreads, smem, stream);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace sample
+}  // namespace detail
+}  // namespace raft_b200

@@ -998,8 +998,8 @@ inline Args<T> rows_from(const Args<T>& a, int64_t r0, int64_t n)
   return b;
 }
 
-template <typename Kernel, typename T>
-inline cudaError_t launch_clusters(Kernel kern, const Args<T>& a, int64_t ctas, int size, int threads, size_t smem,
+template <typename Kernel, typename A>
+inline cudaError_t launch_clusters(Kernel kern, const A& a, int64_t ctas, int size, int threads, size_t smem,
                                    cudaStream_t stream)
 {
   cudaLaunchConfig_t cfg = {};

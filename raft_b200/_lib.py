@@ -44,6 +44,25 @@ class ReduceDesc(ctypes.Structure):
     ]
 
 
+class SampleDesc(ctypes.Structure):
+    """b2r_sample_desc"""
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("out_dtype", ctypes.c_int32),
+        ("n_rows", ctypes.c_int64),
+        ("vocab", ctypes.c_int64),
+        ("ld", ctypes.c_int64),
+        ("temperature", ctypes.c_void_p),
+        ("top_k", ctypes.c_void_p),
+        ("top_p", ctypes.c_void_p),
+        ("min_p", ctypes.c_void_p),
+        ("temperature_all", ctypes.c_float),
+        ("top_k_all", ctypes.c_int32),
+        ("top_p_all", ctypes.c_float),
+        ("min_p_all", ctypes.c_float),
+    ]
+
+
 # every symbol include/raft_b200.h declares: name -> (restype, argtypes)
 _vp, _i32, _i64, _sz, _dbl, _u64 = (ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t,
                                     ctypes.c_double, ctypes.c_uint64)
@@ -69,6 +88,7 @@ SIGNATURES = {
                                         _i64, _i64, _i64, _dbl, _vp]),
     "b2r_topk_distill_grad": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _i32,
                                              _i64, _i64, _i64, _dbl, _vp]),
+    "b2r_sample_tokens": (ctypes.c_int, [ctypes.POINTER(SampleDesc), _vp, _vp, _vp, _vp, _vp]),
     "b2r_column_sum_f32_noalloc": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _dbl, _vp]),
     "b2r_column_sum_f32_noalloc_max_scratch": (_sz, []),
     "b2r_apply_final": (ctypes.c_int, [_vp, _i32, _i64, _i32, _dbl, _vp]),

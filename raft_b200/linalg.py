@@ -573,6 +573,59 @@ def topk_distill_grad(logits, teacher_ids, teacher_logits, lse, grad_loss, tempe
     return grad
 
 
+def _sample_param(value, name, dtype, n, logits):
+    """(tensor or None, value for all rows) of a sampling parameter given as a number or as a tensor."""
+    if isinstance(value, torch.Tensor):
+        _on_device_of(value, name, logits)
+        if value.dtype != dtype or value.numel() != n or not value.is_contiguous():
+            raise ValueError(f"{name} must be a number or contiguous {dtype} of size n_rows")
+        return value.data_ptr(), 0
+    return None, value
+
+
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, logprobs=None,
+                  index_dtype=torch.int32):
+    """One token for every row of logits, from a uniform number in [0, 1) for each row. In the order of falling logits
+    (equal ones by rising token) the first `top_k` are kept (0: all), of those the tokens whose probability is at
+    least `min_p` of the largest, of those the shortest beginning of the order that holds at least `top_p` of their
+    probability; the drawn token is the first kept one, by token number, at which the running probability under
+    `temperature` exceeds uniform times the kept one. temperature <= 0 takes the largest logit.
+
+    logits: [n_rows x vocab] row-major (rows may be strided), float32 / float16 / bfloat16; uniform: float32 [n_rows];
+    the parameters are numbers or vectors of n_rows (int32 for top_k, float32 for the others). NaN logits count as
+    -inf; a row of -inf alone gives -1. Returns (tokens, logprobs): int32 or int64, and the float32 log of the
+    probability with which each token was drawn."""
+    _require_cuda(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError("logits must be a matrix")
+    dt = _VOCAB_DTYPES.get(logits.dtype)
+    if dt is None:
+        raise L.B2RError(L.ERR_UNSUPPORTED, "sample_tokens")
+    n, vocab = logits.shape
+    ldl = _row_stride(logits, "logits")
+    _per_row(uniform, "uniform", n, logits)
+    if out is None:
+        out = torch.empty(n, dtype=index_dtype, device=logits.device)
+    _on_device_of(out, "out", logits)
+    if out.numel() != n or not out.is_contiguous():
+        raise ValueError("out must be contiguous, of size n_rows")
+    ot = _TOKEN_DTYPES.get(out.dtype)
+    if ot is None:
+        raise L.B2RError(L.ERR_UNSUPPORTED, "sample_tokens")
+    logprobs = torch.empty(n, dtype=torch.float32, device=logits.device) if logprobs is None else \
+        _per_row(logprobs, "logprobs", n, logits)
+    temp_ptr, temp = _sample_param(temperature, "temperature", torch.float32, n, logits)
+    k_ptr, k = _sample_param(top_k, "top_k", torch.int32, n, logits)
+    p_ptr, p = _sample_param(top_p, "top_p", torch.float32, n, logits)
+    m_ptr, m = _sample_param(min_p, "min_p", torch.float32, n, logits)
+    desc = L.SampleDesc(dt, ot, n, vocab, ldl, temp_ptr, k_ptr, p_ptr, m_ptr, temp, min(int(k), 0x7fffffff), p, m)
+    with _on(logits.device):
+        st = L.load().b2r_sample_tokens(desc, out.data_ptr(), logprobs.data_ptr(), logits.data_ptr(),
+                                        uniform.data_ptr(), _stream_ptr(logits.device))
+    L.check(st, "b2r_sample_tokens")
+    return out, logprobs
+
+
 def last_kernel_status(device, clear=True):
     """Synchronises `device` and returns L.OK, or L.ERR_TIMEOUT if a bounded wait inside a kernel of any
     earlier call on that device ran out (that call's unfinished floating-point outputs are NaN)."""
