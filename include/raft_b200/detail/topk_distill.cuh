@@ -35,19 +35,6 @@ struct List {
   int id64;  // tokens are int64 (else int32)
   int tdt;   // b2r_dtype of the teacher's logits
   int k;
-
-  B2R_DI int64_t id(int64_t row, int j) const
-  {
-    return id64 ? int64_t(static_cast<const long long*>(ids)[row * ldi + j])
-                : int64_t(static_cast<const int*>(ids)[row * ldi + j]);
-  }
-  B2R_DI float logit(int64_t row, int j) const
-  {
-    const int64_t at = row * ldt + j;
-    if (tdt == 2) return __half2float(static_cast<const __half*>(teacher)[at]);               // B2R_F16
-    if (tdt == 7) return __bfloat162float(static_cast<const __nv_bfloat16*>(teacher)[at]);    // B2R_BF16
-    return static_cast<const float*>(teacher)[at];
-  }
 };
 
 template <typename T>
@@ -342,19 +329,41 @@ B2R_DI bool weigh_list(const int* id, float* y, int k, float inv_t)
   return some;
 }
 
-// Entry j of a row's list. Both loads are under way before either value is looked at.
+// Entry j of a row's list, as it lies in memory: loads under way do not stop the warp until a value is looked at, and a
+// conversion is such a look.
 struct Entry {
-  int64_t token;
-  float y;
+  unsigned lo, hi;  // token (hi: of int64 tokens)
+  unsigned y;       // bits of the teacher's logit
 
   template <typename T>
   B2R_DI void ask(const Args<T>& a, int64_t row, int j)
   {
-    token = a.list.id(row, j);
-    y     = a.list.logit(row, j);
+    if (a.list.id64) {
+      const uint2 t = *reinterpret_cast<const uint2*>(static_cast<const long long*>(a.list.ids) + row * a.list.ldi + j);
+      lo            = t.x;
+      hi            = t.y;
+    } else {
+      lo = static_cast<const unsigned*>(a.list.ids)[row * a.list.ldi + j];
+    }
+    if (a.list.tdt == 0)
+      y = static_cast<const unsigned*>(a.list.teacher)[row * a.list.ldt + j];
+    else
+      y = static_cast<const uint16_t*>(a.list.teacher)[row * a.list.ldt + j];
   }
-  // as weigh_list wants it
-  B2R_DI int id(int vocab) const { return token >= 0 && token < vocab ? int(token) : -1; }
+  template <typename T>
+  B2R_DI int id(const Args<T>& a) const  // -1: not valid
+  {
+    const bool ok = (!a.list.id64 || hi == 0u) && lo < unsigned(a.vocab);
+    return ok ? int(lo) : -1;
+  }
+  template <typename T>
+  B2R_DI float logit(const Args<T>& a) const
+  {
+    if (a.list.tdt == 0) return __uint_as_float(y);
+    if (a.list.tdt == 7) return __uint_as_float(y << 16);  // B2R_BF16
+    const __half_raw h{static_cast<unsigned short>(y)};
+    return __half2float(__half(h));
+  }
 };
 
 // Weight of entry j's token over the whole list (a token may be named more than once); false unless j is the first
@@ -388,8 +397,9 @@ B2R_DI bool listed_weight(const int* id, const float* logp, int k, int j, float*
 // (5000 of 12000 clocks per row in the copies); cluster barriers for the exchange, which wait for the gradient's
 // stores, 1350 us.
 //
-// Two warps work beside the workers, so that no chain of loads is on the workers' path:
-//   the sender   joins the CTA's (m, s), sends the record, issues the copies, and in the first CTA writes the loss;
+// Three warps work beside the workers, so that no chain of loads is on the workers' path:
+//   the sender   joins the CTA's (m, s), sends the record, and in the first CTA writes the loss;
+//   the mover    issues the copies, and waits until a row's gradient has been read before the next row comes in;
 //   the lister   prepares the list of the row after the next: weights, the student's logits of the listed tokens, and
 //                the sums A = sum p (log p - z / T), P = sum p over the tokens this CTA holds, of which the loss is
 //                T^2 (A + P lse). (The listed elements of the gradient are written by the warp that holds them.)
@@ -400,7 +410,7 @@ constexpr int kStages = 3;  // vectors of the row in its second pass, of the nex
 constexpr int kStepNv = 8;  // vectors of a worker, in chunks of four
 
 template <typename T, int NT, bool kEven>
-__global__ void __launch_bounds__(NT + 64)
+__global__ void __launch_bounds__(NT + 96, NT == 256 ? 2 : 1)
 distill_step_kernel(const Args<T> a)
 {
   constexpr int VE = Vec16Of<T>::value;
@@ -419,12 +429,14 @@ distill_step_kernel(const Args<T> a)
   __shared__ double list_sums[3][2];  // A, P
   __shared__ float factor_s[3];       // weight of the row's gradient, 0 for a row without a list
   __shared__ int some_s[3];
+  __shared__ int twice_s[3];  // a token of this CTA's is named twice
   __shared__ int gave_up;
   Vec* stages         = reinterpret_cast<Vec*>(step_smem);                   // [kStages][NT * NV]
   const int k         = a.list.k;
   int* ids            = reinterpret_cast<int*>(stages + kStages * NT * NV);  // [3][k]
   float* logps        = reinterpret_cast<float*>(ids + 3 * k);               // [3][k]
   float* zids         = logps + 3 * k;                                       // [3][k]
+  unsigned* seen      = reinterpret_cast<unsigned*>(zids + 3 * k);           // a bit per element of the part
   const unsigned rank = cluster_rank();
   const unsigned size = cluster_size();
   const int tid       = int(threadIdx.x);
@@ -449,9 +461,11 @@ distill_step_kernel(const Args<T> a)
   // Nobody writes there again, but for rows of different phases, whose parts differ by a vector.
   {
     const RowPart<T> part = part_of(0);
-    for (int i = tid; i < NT * NV; i += NT + 64)
+    for (int i = tid; i < NT * NV; i += NT + 96)
       if (i >= part.n) stages[i] = stages[NT * NV + i] = stages[2 * NT * NV + i] = minus_inf<T>();
   }
+  for (int i = tid; i < NT * NV * VE / 32; i += NT + 96)
+    seen[i] = 0;
   fence_proxy_async();
   __syncthreads();
   cluster_arrive();  // every CTA of the cluster has started, its barriers are set up
@@ -463,6 +477,10 @@ distill_step_kernel(const Args<T> a)
     if (row >= a.n_rows) return;
     const RowPart<T> part = part_of(row);
     Vec* to               = stages + stage * (NT * NV);
+    if (lane == 0 && part.lo != 0) to[0] = part.load_edge(0);
+    if (lane == 1 && part.hi < part.n && (part.n > 1 || part.lo == 0)) to[part.n - 1] = part.load_edge(part.n - 1);
+    if (!kEven && lane == 2 && part.n < NT * NV) to[part.n] = minus_inf<T>();
+    __syncwarp();  // these are there, too, for whoever has seen the barrier
     if (lane == 0) {
       const int whole = part.hi > part.lo ? part.hi - part.lo : 0;
       mbar_expect_tx(&full[stage], unsigned(whole) * 16u);
@@ -470,10 +488,7 @@ distill_step_kernel(const Args<T> a)
         const int n = whole - i < 1024 ? whole - i : 1024;
         bulk_load(to + part.lo + i, part.at + (part.lo + i) * VE, unsigned(n) * 16u, &full[stage]);
       }
-      if (part.lo != 0) to[0] = part.load_edge(0);
     }
-    if (lane == 1 && part.hi < part.n && (part.n > 1 || part.lo == 0)) to[part.n - 1] = part.load_edge(part.n - 1);
-    if (!kEven && lane == 2 && part.n < NT * NV) to[part.n] = minus_inf<T>();
   };
   // the gradient of a row from its buffer to memory, as far as that goes in whole vectors
   auto write_back = [&](int64_t row, int stage) {
@@ -507,46 +522,92 @@ distill_step_kernel(const Args<T> a)
 
   // ---- lister
   const double inverse = 1.0 / a.temperature;
-  auto prepare         = [&](int64_t row, int buf, int stage, unsigned phase) {
+  // The first entries of a row's list and its weight are asked for a turn before they are used, and worked on in
+  // registers; those of long lists behind them go through shared memory.
+  constexpr int kAhead = 4;
+  Entry ahead[kAhead];
+  float ahead_weight = 0.0f;
+  auto ask           = [&](int64_t row) {
+    if (row >= a.n_rows) return;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (u * 32 + lane < k) ahead[u].ask(a, row, u * 32 + lane);
+    ahead_weight = a.grad_loss[row];
+  };
+  auto prepare = [&](int64_t row, int buf, int stage, unsigned phase) {
     if (row >= a.n_rows) return;
     const RowPart<T> part = part_of(row);
-    const float weight    = a.grad_loss[row];
     int* id               = ids + buf * k;
     float* logp           = logps + buf * k;
     float* zid            = zids + buf * k;
-    for (int l0 = 0; l0 < k; l0 += 128) {
-      Entry entry[4];
+    int near_id[kAhead];
+    float near_y[kAhead];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (l0 + u * 32 + lane < k) entry[u].ask(a, row, l0 + u * 32 + lane);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = l0 + u * 32 + lane;
-        if (j < k) {
-          id[j]   = entry[u].id(a.vocab);
-          logp[j] = entry[u].y;
-        }
-      }
+    for (int u = 0; u < kAhead; ++u) {
+      near_id[u] = u * 32 + lane < k ? ahead[u].id(a) : -1;
+      near_y[u]  = ahead[u].logit(a);
     }
-    const bool some = weigh_list(id, logp, k, float(inverse));
+    const float weight = ahead_weight;
+    ask(row + step);
+    for (int j = kAhead * 32 + lane; j < k; j += 32) {
+      Entry entry;
+      entry.ask(a, row, j);
+      id[j]   = entry.id(a);
+      logp[j] = entry.logit(a);
+    }
+    // f(place, token, logit or log weight) for every valid entry; the value may be changed
+    const auto each = [&](auto f) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (near_id[u] >= 0) f(u * 32 + lane, near_id[u], near_y[u]);
+      for (int j = kAhead * 32 + lane; j < k; j += 32)
+        if (id[j] >= 0) f(j, id[j], logp[j]);
+    };
+    const float inv_t = float(inverse);
+    float m           = -INFINITY;
+    bool nan          = false;
+    each([&](int, int, float& y) {
+      m   = fmaxf(m, y);
+      nan = nan || y != y;
+    });
+    m               = warp_max(m);
+    nan             = __any_sync(kFull, nan);
+    const bool some = m > -INFINITY || nan;
+    float total     = 0.0f;
+    each([&](int, int, float& y) { total += some ? expf((y - m) * inv_t) : 0.0f; });
+    const float ls = logf(warp_sum(total));
     // the row itself, for the student's logits of the listed tokens
     const bool here = mbar_wait_bounded(&full[stage], phase, &gave_up, a.ctl.limit_ns);
     const T* held   = reinterpret_cast<const T*>(stages + stage * (NT * NV)) - part.first;  // held[t]: token t
     double sum = 0.0, share = 0.0;
-    for (int j = lane; j < k && some && here; j += 32) {
-      const int t    = id[j];
-      const float lp = logp[j];
-      if (t >= part.token0 && t < part.token1) {
-        const float z  = FloatIo<T>::up(held[t]);
+    bool twice = false;
+    each([&](int j, int t, float& y) {
+      const float lp = some ? (y - m) * inv_t - ls : -INFINITY;
+      logp[j]        = lp;
+      if (t >= part.token0 && t < part.token1 && some && here) {
+        const unsigned at = unsigned(t - part.first), bit = 1u << (at & 31u);
+        twice          = twice || (atomicOr(&seen[at >> 5], bit) & bit) != 0u;
+        const float zt = FloatIo<T>::up(held[t]);
         const double w = double(expf(lp));
-        zid[j]         = z;
-        sum += lp == -INFINITY ? 0.0 : w * (double(lp) - double(z) * inverse);
+        zid[j]         = zt;
+        sum += lp == -INFINITY ? 0.0 : w * (double(lp) - double(zt) * inverse);
         share += w;
       }
+    });
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (u * 32 + lane < k) id[u * 32 + lane] = near_id[u];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(kFull, sum, o);
+      share += __shfl_xor_sync(kFull, share, o);
     }
-    sum   = warp_sum(sum);
-    share = warp_sum(share);
+    twice = __any_sync(kFull, twice);
+    each([&](int, int t, float&) {
+      if (t >= part.token0 && t < part.token1) seen[unsigned(t - part.first) >> 5] = 0;
+    });
     if (lane == 0) {
+      twice_s[buf]      = twice;
       list_sums[buf][0] = here ? sum : double(NAN);
       list_sums[buf][1] = share;
       some_s[buf]       = some;
@@ -609,7 +670,7 @@ distill_step_kernel(const Args<T> a)
     Vec* mine             = stages + stage * (NT * NV) + tid;
     T* to                 = a.grad + row * a.ldg + part.first;
     const bool same       = same_phase(to, part.at);
-    const bool plain      = same && !part.edges();  // nothing goes straight to memory
+    const bool plain      = same && !part.edges();  // everything is written by the bulk copy
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (i * NT + warp * 32 < part.n) {
@@ -619,10 +680,13 @@ distill_step_kernel(const Args<T> a)
         for (int q = 0; q < VE / 2; ++q)
           down2<T>(o, q, mul2(ex2_2(fma2(add2(up2<T>(v, q), sub), mul, off)), fact2));
         if (!some) o = Vec{};
-        const int j = i * NT + tid;
-        if (part.whole(j)) mine[i * NT] = o;
-        if (!plain && j < part.n && !(same && part.whole(j))) part.store_edge(to, j, o);
+        if (i * NT + tid < part.n) mine[i * NT] = o;
       }
+    }
+    if (!plain) {
+#pragma unroll 1
+      for (int j = tid; j < part.n; j += NT)
+        if (!(same && part.whole(j))) part.store_edge(to, j, mine[j - tid]);
     }
     // the listed elements of the warp's vectors: q - sum of the token's weights
     __syncwarp();
@@ -630,9 +694,22 @@ distill_step_kernel(const Args<T> a)
       const int* id     = ids + buf * k;
       const float* logp = logps + buf * k;
       const float* zid  = zids + buf * k;
+      const bool twice  = twice_s[buf] != 0;
       for (int l0 = 0; l0 < k; l0 += 32) {
         const int t0  = l0 + lane < k ? id[l0 + lane] : -1;
         const bool my = t0 >= part.token0 && t0 < part.token1 && (unsigned(t0 - part.first) / VE) % NT / 32 == unsigned(warp);
+        const auto put = [&](int t, float zt, float w) {
+          const T v    = FloatIo<T>::down(fact * (ex2((zt - all.m) * c - l2s) - w));
+          const int at = t - part.first;
+          if (same && part.whole(at / VE))
+            reinterpret_cast<T*>(stages + stage * (NT * NV))[at] = v;
+          else
+            to[at] = v;
+        };
+        if (!twice) {
+          if (my) put(t0, zid[l0 + lane], expf(logp[l0 + lane]));
+          continue;
+        }
         for (unsigned left = __ballot_sync(kFull, my); left != 0u; left &= left - 1u) {
           const int j = l0 + __ffs(int(left)) - 1;
           const int t = id[j];
@@ -645,26 +722,23 @@ distill_step_kernel(const Args<T> a)
             }
           }
           w = warp_sum(w);
-          if (!__any_sync(kFull, before != 0) && lane == 0) {
-            const T v    = FloatIo<T>::down(fact * (ex2((zid[j] - all.m) * c - l2s) - w));
-            const int at = t - part.first;
-            if (same && part.whole(at / VE))
-              reinterpret_cast<T*>(stages + stage * (NT * NV))[at] = v;
-            else
-              to[at] = v;
-          }
+          if (!__any_sync(kFull, before != 0) && lane == 0) put(t, zid[j], w);
         }
       }
     }
     fence_proxy_async();
   };
 
+  // workers and sender
+  const auto handover = [] { asm volatile("bar.sync 1, %0;" ::"n"(NT + 32) : "memory"); };
+
   // Row number n of this cluster lies in buffer n % 3, as does its list; its records at n & 3.
-  if (warp == NW) {
+  if (warp == NW + 2) {
     for (int n = 0; n < kStages; ++n)
       request(first + n * step, n);
   }
   __syncthreads();
+  if (warp == NW + 1) ask(first);
   if (warp == NW + 1) prepare(first, 0, 0, 0);
   if (warp == NW + 1) prepare(first + step, 1, 1, 0);
   if (warp < NW) first_pass(part_of(first).n, 0, 0);
@@ -680,12 +754,27 @@ distill_step_kernel(const Args<T> a)
     const unsigned nround = nxt == 0 ? round ^ 1u : round;
     const int nn          = nxt + 1 == kStages ? 0 : nxt + 1;
     const unsigned phase  = unsigned(n >> 2) & 1u;  // of the records
-    if (warp < NW && row + step < a.n_rows) first_pass(part_of(row + step).n, nxt, nround);
-    __syncthreads();
+    bool listed = false;
     if (warp < NW) {
+      if (row + step < a.n_rows) first_pass(part_of(row + step).n, nxt, nround);
+      handover();
       second_pass(row, n, cur, cur, phase);
     } else if (warp == NW) {
+      handover();
       if (row + step < a.n_rows && there) send(n + 1, nxt);
+      listed = some_s[cur] != 0;
+    } else if (warp == NW + 1 && there) {
+      // (the list of the row after the next goes where the row before had its)
+      prepare(row + 2 * step, nn, nn, nn == 0 || nxt == 0 ? round ^ 1u : round);
+    }
+    __syncthreads();
+    if (warp == NW + 2) {
+      write_back(row, cur);
+      bulk_store_wait_read();  // (by the lane that stores)
+      __syncwarp();
+      // (after a give-up nothing says that the buffer's last copy has landed)
+      if (*static_cast<volatile int*>(&gave_up) == 0) request(row + 3 * step, cur);
+    } else if (warp == NW) {
       there = there && mbar_wait_bounded(&arrived[n & 3], phase, &gave_up, a.ctl.limit_ns);
       if (rank == 0) {
         const float4 r   = lane < int(size) ? record[n & 3][lane] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
@@ -696,27 +785,15 @@ distill_step_kernel(const Args<T> a)
         const double wgt = warp_sum(p);
         const double lse = there ? double(all.m) * inverse + double(logf(all.s)) : double(NAN);
         if (lane == 0) {
-          if (a.loss != nullptr)
-            a.loss[row] = some_s[cur] != 0 ? float((sum + wgt * lse) * a.temperature * a.temperature) : 0.0f;
+          if (a.loss != nullptr) a.loss[row] = listed ? float((sum + wgt * lse) * a.temperature * a.temperature) : 0.0f;
           if (a.lse != nullptr) a.lse[row] = float(lse);
         }
       }
-    } else if (there) {
-      // (the buffer of this row's successor's successor: its list goes where the row before had its)
-      prepare(row + 2 * step, nn, nn, nn == 0 || nxt == 0 ? round ^ 1u : round);
-    }
-    __syncthreads();
-    if (warp == NW) {
-      write_back(row, cur);
-      bulk_store_wait_read();  // (by the lane that stores)
-      __syncwarp();
-      // (after a give-up nothing says that the buffer's last copy has landed)
-      if (there && *static_cast<volatile int*>(&gave_up) == 0) request(row + 3 * step, cur);
     }
     cur   = nxt;
     round = nround;
   }
-  if (warp == NW) {
+  if (warp == NW + 2) {
     bulk_store_wait_all();
     if (*static_cast<volatile int*>(&gave_up) != 0 && lane == 0) {
       // copies still on their way in must have landed before the CTA leaves: the last of each buffer, if any
@@ -770,10 +847,10 @@ distill_stream_kernel(const Args<T> a)
       for (int j = lane; j < k; j += 32) {
         Entry entry;
         entry.ask(a, row, j);
-        const int at = entry.id(a.vocab);
+        const int at = entry.id(a);
         id[j]        = at;
         zid[j]       = at >= 0 ? FloatIo<T>::up(z[at]) : 0.0f;
-        logp[j]      = entry.y;
+        logp[j]      = entry.logit(a);
       }
       const bool some = weigh_list(id, logp, k, float(1.0 / a.temperature));
       if (lane == 0) some_s = some;
@@ -931,10 +1008,10 @@ distill_grad_kernel(const Args<T> a, unsigned parts)
     for (int j = tid - NT; j < k; j += 32) {
       Entry entry;
       entry.ask(a, row, j);
-      const int at = entry.id(a.vocab);
+      const int at = entry.id(a);
       id[j]        = at;
       zid[j]       = at >= part.token0 && at < part.token1 ? FloatIo<T>::up(z[at]) : 0.0f;
-      logp[j]      = entry.y;
+      logp[j]      = entry.logit(a);
     }
     const bool some = weigh_list(id, logp, k, float(1.0 / a.temperature));
     if (tid == NT) some_s = some;
@@ -1059,13 +1136,13 @@ template <typename T, int NT, bool kEven>
 inline cudaError_t launch_step_as(Args<T> a, int64_t most, int size, cudaStream_t stream)
 {
   auto kern         = distill_step_kernel<T, NT, kEven>;
-  const size_t smem = size_t(kStages) * NT * kStepNv * 16 + size_t(a.list.k) * 36;
+  const size_t smem = size_t(kStages) * NT * kStepNv * 16 + size_t(a.list.k) * 36 + NT * kStepNv * Vec16Of<T>::value / 8;
   a.per_cta         = int(ceil_div<int64_t>(most, size));
   cudaError_t e     = ensure_dynamic_smem(kern, smem);
   if (e != cudaSuccess) return e;
-  const int64_t fit      = resident_clusters(kern, size, NT + 64, smem);
+  const int64_t fit      = resident_clusters(kern, size, NT + 96, smem);
   const int64_t clusters = a.n_rows < fit ? a.n_rows : fit;
-  return launch_clusters(kern, a, clusters * size, size, NT + 64, smem, stream);
+  return launch_clusters(kern, a, clusters * size, size, NT + 96, smem, stream);
 }
 
 template <typename T, int NT>
@@ -1098,7 +1175,7 @@ template <typename T>
 inline cudaError_t launch_loss_and_grad(const Args<T>& a, cudaStream_t stream)
 {
   const int64_t most = most_vectors(a);
-  if (a.list.k > 900) return launch_stream<T, 256, true>(a, most, 8, stream);
+  if (a.list.k > 800) return launch_stream<T, 256, true>(a, most, 8, stream);
   if (most <= 64 * kStepNv) return launch_step<T, 64>(a, most, 1, stream);
   if (most <= 256 * kStepNv) return launch_step<T, 256>(a, most, 1, stream);
   for (int size = 1; size <= 8; size *= 2)
