@@ -7,12 +7,15 @@
 // largest logit (the lowest token of equals). NaN logits count as -inf; a row of nothing else has no token: -1.
 //
 // Which side of a border a token falls on is decided by sums over the vocabulary in which a token may weigh 1e-6 of
-// the whole, so weights are computed in fp64 and summed as INTEGERS of 2^-shift, shift = 62 - ceil(log2 vocab) (45 bits
-// for 131072 tokens): exact, the same whatever the order, the split of the row or the number of rows of the call.
+// the whole, so weights are computed in fp64 and summed as INTEGERS of 2^-shift, shift = 62 - ceil(log2 vocab) but at
+// most kMaxShift (45 bits for 131072 tokens): exact, the same whatever the order, the split of the row or the number of rows of the call.
 //
-// A cluster of CTAs takes a row, every CTA a part, which it keeps in shared memory. Thresholds in the order are found
-// by radix selection on the logits' bits, made to rise with their value: histograms of counts (top-k) or of weights
-// (top-p), summed over the cluster through distributed shared memory, a digit at a time.
+// A cluster of CTAs takes a row, every CTA a part, which it keeps in shared memory. The logits' bits, made to rise with
+// their value, are counted by their first kDigitBits while the row comes in; with a top-k or a min-p, or from the
+// weights of those bins for a top-p, that bounds the beginning of the order that can be kept. Where it is short (at
+// most kList tokens: nearly always) it is collected in the first CTA, sorted, and the rest happens there; the others
+// are done. Long ones (a flat distribution, a large k) are narrowed by radix selection, a digit at a time, by counts or
+// weights summed over the cluster through distributed shared memory, and drawn from in place.
 #pragma once
 
 #include "launch.cuh"
@@ -31,6 +34,8 @@ constexpr int kMaxCluster = 8;
 constexpr int kDigitBits  = 11;
 constexpr int kBins       = 1 << kDigitBits;
 constexpr int kMaxPartKb  = 160;  // of a row in a CTA's shared memory
+constexpr int kList       = 2048;
+constexpr int kMaxShift   = 50;  // weights below 2^51, so that an addition rounds them to integers
 
 template <typename T>
 struct Args {
@@ -144,6 +149,29 @@ B2R_DI unsigned cluster_load_u32(const unsigned* p, unsigned rank)
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
   return v;
 }
+B2R_DI unsigned cluster_address(const void* p, unsigned rank)
+{
+  unsigned remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(p)), "r"(rank));
+  return remote;
+}
+B2R_DI void cluster_add_u32(unsigned* p, unsigned rank, unsigned v)
+{
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_address(p, rank)), "r"(v) : "memory");
+}
+B2R_DI void cluster_max_u32(unsigned* p, unsigned rank, unsigned v)
+{
+  asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(cluster_address(p, rank)), "r"(v) : "memory");
+}
+B2R_DI unsigned cluster_fetch_add_u32(unsigned* p, unsigned rank, unsigned v)
+{
+  unsigned old;
+  asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;"
+               : "=r"(old)
+               : "r"(cluster_address(p, rank)), "r"(v)
+               : "memory");
+  return old;
+}
 B2R_DI void cluster_sync()
 {
   distill::cluster_arrive();
@@ -157,8 +185,11 @@ sample_kernel(const Args<T> a)
   constexpr int VE = Vec16Of<T>::value;
   using K          = Key<T>;
   extern __shared__ __align__(16) unsigned char sample_smem[];
-  __shared__ unsigned hist[2][kBins];           // low and high words of the bins' sums
-  __shared__ u64 bins[kBins];                   // sums over the cluster of the bins this CTA looks after
+  __shared__ unsigned hist[2][kBins];           // counts of this CTA; low and high words of the bins' sums
+  __shared__ unsigned totals[kBins];            // counts of the row
+  __shared__ __align__(16) u64 bins[kBins];     // sums over the cluster of the bins this CTA looks after
+  __shared__ double powers[32];                 // 2^(i / 32)
+  __shared__ unsigned kmax_all, list_n, list_at, list_base;
   __shared__ u64 posted[4][kMaxCluster];        // a value from every CTA of the cluster, four exchanges deep
   __shared__ u64 result[2][2];
   __shared__ u64 warp_part[kWarps];
@@ -168,6 +199,11 @@ sample_kernel(const Args<T> a)
   const unsigned rank = distill::cluster_rank();
   const unsigned size = distill::cluster_size();
   const int tid = int(threadIdx.x), warp = tid >> 5, lane = tid & 31;
+  for (int i = tid; i < kBins; i += kThreads)
+    hist[0][i] = totals[i] = 0;
+  if (tid < 32) powers[tid] = exp2(double(tid) * 0.03125);
+  if (tid == 0) kmax_all = list_n = list_at = 0;
+  __syncthreads();
   distill::cluster_arrive();
   grid_dep_sync();
 
@@ -203,26 +239,37 @@ sample_kernel(const Args<T> a)
     return s;
   };
 
-  // the row, and its largest key
-  unsigned kmax = 0;
+  // the row, its largest key, and (where anything is to be left out) the counts by the first digit
+  const bool by_k    = !greedy && top_k > 0 && top_k < a.vocab;
+  const bool by_p    = !greedy && top_p < 1.0f;
+  const bool by_min  = !greedy && min_p > 0.0f;
+  const bool counted = by_k || by_p || by_min;
+  constexpr int kLow = K::kBits - kDigitBits;  // bits behind the first digit
+  unsigned kmax      = 0;
   for (int j = tid; j < part.n; j += kThreads) {
     const Words4 v = part.load(j);
     if (kCached) slice[j] = v;
 #pragma unroll
-    for (int e = 0; e < VE; ++e)
-      kmax = max(kmax, K::of(v, e));
+    for (int e = 0; e < VE; ++e) {
+      const unsigned key = K::of(v, e);
+      kmax               = max(kmax, key);
+      if (counted && key > K::kNegInf) atomicAdd(&hist[0][key >> kLow], 1u);
+    }
   }
   kmax = __reduce_max_sync(distill::kFull, kmax);
-  if (lane == 0) warp_part[warp] = kmax;
   __syncthreads();
-  for (int w = 0; w < kWarps; ++w)
-    kmax = max(kmax, unsigned(warp_part[w]));
   distill::cluster_wait();
-  {
-    const u64* all = post(kmax);
-    for (unsigned r = 0; r < size; ++r)
-      kmax = max(kmax, unsigned(all[r]));
+  if (lane < int(size)) cluster_max_u32(&kmax_all, unsigned(lane), kmax);
+  if (counted) {
+    for (int i = tid; i < kBins; i += kThreads) {
+      const unsigned n = hist[0][i];
+      if (n != 0)
+        for (unsigned r = 0; r < size; ++r)
+          cluster_add_u32(&totals[i], r, n);
+    }
   }
+  cluster_sync();
+  kmax = kmax_all;
   auto write = [&](int64_t token, float logprob) {  // by one thread of the cluster
     if (a.out64)
       static_cast<long long*>(a.out)[row] = token;
@@ -236,11 +283,25 @@ sample_kernel(const Args<T> a)
   }
   const double zmax  = double(K::value(kmax));
   const double slope = 1.4426950408889634 / double(temp);
-  const double unit  = double(u64(1) << a.shift);
-  const auto weight  = [&](unsigned key) -> u64 {
-    if (key == kmax) return u64(1) << a.shift;
-    const double x = (double(K::value(key)) - zmax) * slope;
-    return x <= 0.0 ? u64(__double2ull_rn(exp2(x) * unit)) : 0;  // (0 for -inf * 0: a +inf logit at infinite temperature)
+  // 2^x by table and polynomial: x * 32 = n + r, 2^x = 2^(n / 32) 2^(r / 32), the second by its Taylor series to the
+  // fifth power (|r / 32| <= 1 / 64: 3e-15), the first from `powers` and an exponent (P. T. P. Tang, 1989)
+  const double slope32 = slope * 32.0;
+  const int shift      = a.shift;
+  const auto weight    = [&](unsigned key) -> u64 {
+    if (key == kmax) return u64(1) << shift;
+    const double y = (double(K::value(key)) - zmax) * slope32;
+    if (!(y > -32.0 * double(kMaxShift + 2))) return 0;  // (and -inf * 0: a +inf logit at infinite temperature)
+    const double big = y + 6755399441055744.0;           // 1.5 * 2^52: the nearest integer in the low bits
+    const int n      = __double2loint(big);
+    const double r   = (y - (big - 6755399441055744.0)) * (0.6931471805599453 / 32.0);
+    double p         = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    p                = fma(p, r, 1.0 / 6.0);
+    p                = fma(p, r, 0.5);
+    p                = fma(p, r, 1.0);
+    p                = fma(p, r, 1.0);
+    const double w   = p * powers[n & 31];
+    const double s   = __hiloint2double(__double2hiint(w) + (((n >> 5) + shift) << 20), __double2loint(w));
+    return u64(__double_as_longlong(s + 4503599627370496.0)) & 0xfffffffffffffull;  // 2^52: rounds to an integer
   };
 
   // kept: key > tau, or key == tau and token <= last
@@ -326,14 +387,15 @@ sample_kernel(const Args<T> a)
   };
   // The border of the order at which the sum of value(key) over the kept tokens reaches `target` (at least 1, at most
   // the whole sum): its key in *border, the sum over larger keys in *above. With kCount the values are 1.
-  // A target above the whole sum, which is returned in *total: the border is below every kept key, false.
-  auto select = [&](auto count, auto value, auto target_of, unsigned* border, u64* above, u64* total) {
+  // A target above the whole sum, which is returned in *total: the border is below every kept key, false. With fewer
+  // `digits` than keys have, the border's first ones.
+  auto select = [&](auto count, auto value, auto target_of, int digits, unsigned* border, u64* above, u64* total) {
     constexpr bool kCount = decltype(count)::value;
     unsigned prefix = 0;  // bits of the border found so far
     int left        = K::kBits;
     u64 over        = 0;
     u64 target      = 0;
-    while (left > 0) {
+    while (left > 0 && digits-- > 0) {
       const int bits  = left > kDigitBits ? kDigitBits : left;
       const int shift = left - bits;
       const int n     = 1 << bits;
@@ -449,24 +511,208 @@ sample_kernel(const Args<T> a)
     }
     return;
   }
-  if (top_k > 0 && top_k < a.vocab) {
+  // The lowest bin of the first digit that can hold kept tokens, and the number of tokens from it up.
+  // w >= min_p, as a bound on the key
+  const double mp     = min_p < 1.0f ? double(min_p) : 1.0;
+  const unsigned kmin = !by_min ? 0u : (mp == 1.0 ? kmax : min(kmax, K::at_least(zmax + log2(mp) / slope)));
+  const auto tokens_from = [&](const unsigned* counts, unsigned bin) {
+    u64 s = 0;
+    for (int i = tid; i < kBins; i += kThreads)
+      s += unsigned(i) >= bin ? counts[i] : 0u;
+    return block_sum(s);
+  };
+  // Draws from the tokens of the bins from `bin` up, all of whose n are collected in the first CTA. `whole`: the weight
+  // of all tokens that top-p is measured by, or 0: that of the first top_k and min-p leave.
+  auto draw_from_list = [&](unsigned bin, int n, u64 whole) {
+    const u64 own = tokens_from(hist[0], bin);
+    if (tid == 0) list_base = cluster_fetch_add_u32(&list_n, 0, unsigned(own));
+    __syncthreads();
+    for (int j = tid; j < part.n && own != 0; j += kThreads) {
+      const Words4 v = vec(j);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const unsigned key = K::of(v, e);
+        if (key > K::kNegInf && (key >> kLow) >= bin) {
+          const unsigned token = unsigned(part.first + j * VE + e);
+          // larger keys first, lower tokens first among equals
+          cluster_store_u64(&bins[list_base + atomicAdd(&list_at, 1u)], 0, (u64(key) << 32) | (0xffffffffu - token));
+        }
+      }
+    }
+    cluster_sync();
+    if (rank != 0) return;
+    u64* list    = bins;
+    u64* weights = reinterpret_cast<u64*>(&hist[0][0]);  // [kList]
+    // falling order of list[0 .. n)
+    const auto sort = [&](int count) {
+      int padded = 32;
+      while (padded < count)
+        padded *= 2;
+      for (int i = count + tid; i < padded; i += kThreads)
+        list[i] = 0;
+      for (int k = 2; k <= padded; k *= 2) {
+        for (int h = k / 2; h > 0; h /= 2) {
+          __syncthreads();
+          for (int i = tid; i < padded / 2; i += kThreads) {
+            const int lo = 2 * i - (i & (h - 1)), hi = lo + h;
+            const u64 x = list[lo], y = list[hi];
+            if ((x < y) == ((lo & k) == 0)) {
+              list[lo] = y;
+              list[hi] = x;
+            }
+          }
+        }
+      }
+      __syncthreads();
+    };
+    sort(n);
+    int m = by_k && top_k < n ? top_k : n;
+    // running weights of the first m that min-p leaves (from it on all are below): four places per thread
+    constexpr int kEach = kList / kThreads;
+    const auto running  = [&](auto value) {  // inclusive sums over the places into `weights`, the whole one returned
+      u64 v[kEach], s = 0;
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) {
+        const int i = tid * kEach + q;
+        s += i < m ? value(i) : 0;
+        v[q] = s;
+      }
+      const u64 incl = warp_scan_u64(s);
+      __syncthreads();
+      if (lane == 31) warp_part[warp] = incl;
+      __syncthreads();
+      u64 base = incl - s, sum = 0;
+      for (int w = 0; w < kWarps; ++w) {
+        base += w < warp ? warp_part[w] : 0;
+        sum += warp_part[w];
+      }
+#pragma unroll
+      for (int q = 0; q < kEach; ++q)
+        weights[tid * kEach + q] = base + v[q];
+      __syncthreads();
+      return sum;
+    };
+    const auto key_at = [&](int i) { return unsigned(list[i] >> 32); };
+    u64 total         = running([&](int i) { return key_at(i) >= kmin ? weight(key_at(i)) : 0; });
+    if (by_min) {
+      u64 left = 0;
+      for (int i = tid; i < m; i += kThreads)
+        left += key_at(i) >= kmin ? 1 : 0;
+      m = int(block_sum(left));
+    }
+    if (by_p) {
+      const u64 of = whole != 0 ? whole : total;
+      const double t = ceil(double(top_p) * double(of));
+      u64 target     = t >= 1.0 ? u64(t) : 1;
+      if (target > of) target = of;
+      u64 below = 0;  // places before the one at which the weight reaches the target
+      for (int i = tid; i < m; i += kThreads)
+        below += weights[i] < target ? 1 : 0;
+      below = block_sum(below);
+      m     = below + 1 < u64(m) ? int(below) + 1 : m;
+      total = weights[m - 1];
+    }
+    const double t = double(u) * double(total);
+    u64 target     = t > 0.0 ? u64(t) : 0;
+    if (target >= total) target = total - 1;
+    const auto done = [&](int token, unsigned key) {
+      write(token, float(log(double(weight(key)) / double(total))));
+    };
+    if (m <= 128) {  // every place sums the weights of lower tokens itself
+      if (tid < m) {
+        const u64 mine = list[tid];
+        u64 before     = 0;
+        for (int i = 0; i < m; ++i) {
+          const u64 w = weights[i] - (i > 0 ? weights[i - 1] : 0);
+          before += unsigned(list[i]) > unsigned(mine) ? w : 0;  // (the complement of the token)
+        }
+        const u64 w = weights[tid] - (tid > 0 ? weights[tid - 1] : 0);
+        if (before <= target && target < before + w) done(int(0xffffffffu - unsigned(mine)), unsigned(mine >> 32));
+      }
+      return;
+    }
+    __syncthreads();
+    for (int i = tid; i < m; i += kThreads)
+      list[i] = (list[i] << 32) | (list[i] >> 32);  // complements of tokens fall where tokens rise
+    __syncthreads();
+    sort(m);
+    (void)running([&](int i) { return weight(unsigned(list[i])); });
+    for (int i = tid; i < m; i += kThreads)
+      if (weights[i] > target && (i == 0 || weights[i - 1] <= target))
+        done(int(0xffffffffu - unsigned(list[i] >> 32)), unsigned(list[i]));
+  };
+  if (by_k || by_min) {
+    unsigned bin = kmin >> kLow;
+    if (by_k) {  // the bin at which the counts, from the largest keys down, reach top_k
+      constexpr int kEach = kBins / kThreads;
+      const int top       = kBins - 1 - tid * kEach;
+      u64 s               = 0;
+#pragma unroll
+      for (int q = 0; q < kEach; ++q)
+        s += totals[top - q];
+      const u64 incl = warp_scan_u64(s);
+      if (lane == 31) warp_part[warp] = incl;
+      if (tid == 0) carry = 0;
+      __syncthreads();
+      u64 run = incl - s;
+      for (int w = 0; w < warp; ++w)
+        run += warp_part[w];
+      if (run < u64(top_k) && u64(top_k) <= run + s) {
+        int q = 0;
+        while ((run += totals[top - q]) < u64(top_k))
+          ++q;
+        carry = u64(top - q);
+      }
+      __syncthreads();
+      bin = max(bin, unsigned(carry));
+    }
+    const u64 n = tokens_from(totals, bin);
+    if (n <= kList) {
+      draw_from_list(bin, int(n), 0);
+      return;
+    }
+  } else if (by_p) {
+    unsigned bin;
+    u64 above, whole;
+    const auto target_of = [&](u64 sum) {
+      const double t = ceil(double(top_p) * double(sum));
+      const u64 goal = t >= 1.0 ? u64(t) : 1;
+      return goal < sum ? goal : sum;
+    };
+    (void)select(std::false_type{}, weight, target_of, 1, &bin, &above, &whole);
+    const u64 n = tokens_from(totals, bin);
+    if (n <= kList) {
+      // (the histogram has been used for weights: this CTA's counts again)
+      __syncthreads();
+      for (int i = tid; i < kBins; i += kThreads)
+        hist[0][i] = 0;
+      __syncthreads();
+      for (int j = tid; j < part.n; j += kThreads) {
+        const Words4 v = vec(j);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const unsigned key = K::of(v, e);
+          if (key > K::kNegInf && (key >> kLow) >= bin) atomicAdd(&hist[0][key >> kLow], 1u);
+        }
+      }
+      __syncthreads();
+      draw_from_list(bin, int(n), whole);
+      return;
+    }
+  }
+  if (by_k) {
     unsigned border;
     u64 above, total;
-    if (select(std::true_type{}, weight, [&](u64) { return u64(top_k); }, &border, &above, &total)) {
+    if (select(std::true_type{}, weight, [&](u64) { return u64(top_k); }, 4, &border, &above, &total)) {
       tau = border;
       limit_ties(u64(top_k) - above);
     }
   }
-  if (min_p > 0.0f) {
-    // w >= min_p, as a bound on the logit
-    const double p     = min_p < 1.0f ? double(min_p) : 1.0;
-    const unsigned low = p == 1.0 ? kmax : K::at_least(zmax + log2(p) / slope);
-    if (low > tau) {
-      tau  = low < kmax ? low : kmax;
-      last = 0x7fffffff;
-    }
+  if (by_min && kmin > tau) {
+    tau  = kmin;
+    last = 0x7fffffff;
   }
-  if (top_p < 1.0f) {
+  if (by_p) {
     unsigned border;
     u64 above, total, target = 1;
     const auto target_of = [&](u64 whole) {
@@ -475,7 +721,7 @@ sample_kernel(const Args<T> a)
       if (target > whole) target = whole;
       return target;
     };
-    if (select(std::false_type{}, weight, target_of, &border, &above, &total)) {
+    if (select(std::false_type{}, weight, target_of, 4, &border, &above, &total)) {
       const bool same = border == tau;
       const u64 w     = weight(border);
       tau             = border;
@@ -513,7 +759,7 @@ inline cudaError_t launch_sample(Args<T> a, cudaStream_t stream)
                                 (a.n_rows * size < 2 * int64_t(sm_count()) && most > int64_t(size) * 512)))
     size *= 2;
   a.per_cta         = int(ceil_div<int64_t>(most > 0 ? most : 1, size));
-  a.shift           = 62;
+  a.shift           = kMaxShift;
   while (a.shift > 0 && (int64_t(1) << (62 - a.shift)) < a.vocab)
     --a.shift;
   const bool cached  = int64_t(a.per_cta) * 16 <= int64_t(kMaxPartKb) * 1024;
