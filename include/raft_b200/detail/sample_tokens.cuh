@@ -11,15 +11,18 @@
 // most kMaxShift (45 bits for 131072 tokens): exact, the same whatever the order, the split of the row or the number of rows of the call.
 //
 // A cluster of CTAs takes a row, every CTA a part, which it keeps in shared memory. The logits' bits, made to rise with
-// their value, are counted by their first kDigitBits while the row comes in; with a top-k or a min-p, or from the
-// weights of those bins for a top-p, that bounds the beginning of the order that can be kept. Where it is short (at
-// most kList tokens: nearly always) it is collected in the first CTA, sorted, and the rest happens there; the others
-// are done. Long ones (a flat distribution, a large k) are narrowed by radix selection, a digit at a time, by counts or
-// weights summed over the cluster through distributed shared memory, and drawn from in place.
+// their value, are counted by their first kDigitBits as soon as the row has come in, and the counts bound the beginning
+// of the order that can be kept: by top_k, by the bin of the lowest logit that min_p admits, or, for a top-p alone, by
+// taking a beginning of at most kShort or kList tokens and looking whether its weight is enough. It is collected in the
+// first CTA, sorted, and the rest happens there; the others are done. Longer beginnings (a flat distribution, a large k)
+// are narrowed by radix selection, a digit at a time, by counts or weights summed over the cluster through distributed
+// shared memory, and drawn from in place.
 #pragma once
 
 #include "launch.cuh"
 #include "topk_distill.cuh"  // RowPart, cluster primitives
+
+#include <cfloat>
 
 namespace raft_b200 {
 namespace detail {
@@ -35,6 +38,7 @@ constexpr int kDigitBits  = 11;
 constexpr int kBins       = 1 << kDigitBits;
 constexpr int kMaxPartKb  = 160;  // of a row in a CTA's shared memory
 constexpr int kList       = 2048;
+constexpr int kShort      = 512;  // sorted by counting, a token per thread
 constexpr int kMaxShift   = 50;  // weights below 2^51, so that an addition rounds them to integers
 
 template <typename T>
@@ -58,64 +62,85 @@ struct Args {
   int shift;    // weights are integers of 2^-shift
 };
 
-// The bits of an element as a number that rises with its value: -0 as +0, NaN as -inf.
-template <typename T>
-struct Key;
-template <>
-struct Key<float> {
-  static constexpr int kBits        = 32;
-  static constexpr unsigned kNegInf = 0x007fffffu;
-  B2R_DI static unsigned of(const Words4& v, int e)
+// An element as an unsigned number of its own width that rises with its value: half the range plus or minus the bits
+// of its magnitude, so that -0 and +0 are one; NaN as -inf. Keys are packed as the elements were.
+template <typename T, int kBits_, unsigned kInf>
+struct KeyOf {
+  static constexpr int kBits        = kBits_;
+  static constexpr unsigned kZero   = 1u << (kBits - 1);
+  static constexpr unsigned kNegInf = kZero - kInf;
+
+  B2R_DI static unsigned of_bits(unsigned b)  // bits of an element
   {
-    const unsigned b = v.w[e];
-    if ((b & 0x7fffffffu) > 0x7f800000u) return kNegInf;
-    return (b & 0x80000000u) ? (b == 0x80000000u ? 0x80000000u : ~b) : (b | 0x80000000u);
+    const unsigned mag = b & (kZero - 1u);
+    const unsigned key = (b & kZero) ? kZero - mag : kZero + mag;
+    return mag > kInf ? kNegInf : key;
   }
-  B2R_DI static float value(unsigned k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+  B2R_DI static Words4 pack(const Words4& v)
+  {
+    Words4 r;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      r.w[q] = kBits == 32 ? of_bits(v.w[q]) : (of_bits(v.w[q] & 0xffffu) | (of_bits(v.w[q] >> 16) << 16));
+    return r;
+  }
+  B2R_DI static unsigned at(const Words4& v, int e)
+  {
+    if constexpr (kBits == 32)
+      return v.w[e];
+    else
+      return (e & 1) ? v.w[e / 2] >> 16 : v.w[e / 2] & 0xffffu;
+  }
+  B2R_DI static float value(unsigned k)
+  {
+    const int d         = int(k - kZero);
+    const unsigned bits = d < 0 ? (unsigned(-d) | kZero) : unsigned(d);
+    if constexpr (kBits == 32) {
+      return __uint_as_float(bits);
+    } else {
+      const uint16_t b = uint16_t(bits);
+      T x;
+      memcpy(&x, &b, 2);
+      return FloatIo<T>::up(x);
+    }
+  }
   // lowest key whose value is at least x
   B2R_DI static unsigned at_least(double x)
   {
-    const float f = __double2float_ru(x);
-    Words4 v;
-    v.w[0] = __float_as_uint(f);
-    return of(v, 0);
-  }
-};
-template <typename T, unsigned Inf>
-struct Key16 {
-  static constexpr int kBits        = 16;
-  static constexpr unsigned kNegInf = 0x7fffu - Inf;  // ~(0x8000 | Inf) in 16 bits
-  B2R_DI static unsigned of_bits(unsigned b)
-  {
-    if ((b & 0x7fffu) > Inf) return kNegInf;
-    return (b & 0x8000u) ? (b == 0x8000u ? 0x8000u : (~b & 0xffffu)) : (b | 0x8000u);
-  }
-  B2R_DI static unsigned of(const Words4& v, int e) { return of_bits((e & 1) ? v.w[e / 2] >> 16 : v.w[e / 2] & 0xffffu); }
-  B2R_DI static float value(unsigned k)
-  {
-    const uint16_t b = uint16_t((k & 0x8000u) ? (k & 0x7fffu) : ~k);
-    T x;
-    memcpy(&x, &b, 2);
-    return FloatIo<T>::up(x);
-  }
-  // lowest key whose value is at least x: by bisection of the keys, whose values rise
-  B2R_DI static unsigned at_least(double x)
-  {
-    unsigned lo = kNegInf, hi = 0x8000u + Inf;  // -inf ... +inf
-    while (lo < hi) {
-      const unsigned mid = (lo + hi) >> 1;
-      if (double(value(mid)) >= x)
-        hi = mid;
-      else
-        lo = mid + 1;
+    if constexpr (kBits == 32) {
+      return of_bits(__float_as_uint(__double2float_ru(x)));
+    } else {  // by bisection of the keys, whose values rise
+      unsigned lo = kNegInf, hi = kZero + kInf;  // -inf ... +inf
+      while (lo < hi) {
+        const unsigned mid = (lo + hi) >> 1;
+        if (double(value(mid)) >= x)
+          hi = mid;
+        else
+          lo = mid + 1;
+      }
+      return lo;
     }
-    return lo;
   }
 };
+template <typename T>
+struct Key;
 template <>
-struct Key<__half> : Key16<__half, 0x7c00u> {};
+struct Key<float> : KeyOf<float, 32, 0x7f800000u> {};
 template <>
-struct Key<__nv_bfloat16> : Key16<__nv_bfloat16, 0x7f80u> {};
+struct Key<__half> : KeyOf<__half, 16, 0x7c00u> {};
+template <>
+struct Key<__nv_bfloat16> : KeyOf<__nv_bfloat16, 16, 0x7f80u> {};
+
+// 2^(i / 32)
+__constant__ const double kPowers[32] = {
+  1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237,
+  1.0905077326652577, 1.1143867425958924, 1.1387886347566916, 1.1637248587775775,
+  1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332,
+  1.2968395546510096, 1.3252366431597413, 1.3542555469368927, 1.383909881963832,
+  1.4142135623730951, 1.4451808069770467, 1.4768261459394993, 1.5091644275934228,
+  1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.645755478153965,
+  1.681792830507429, 1.718619298122478, 1.7562521603732995, 1.7947090750031072,
+  1.8340080864093424, 1.8741676341103, 1.9152065613971474, 1.9571441241754002};
 
 B2R_DI u64 warp_sum_u64(u64 v)
 {
@@ -179,49 +204,68 @@ B2R_DI void cluster_sync()
 }
 
 template <typename T, bool kCached>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
 sample_kernel(const Args<T> a)
 {
   constexpr int VE = Vec16Of<T>::value;
   using K          = Key<T>;
   extern __shared__ __align__(16) unsigned char sample_smem[];
-  __shared__ unsigned hist[2][kBins];           // counts of this CTA; low and high words of the bins' sums
-  __shared__ unsigned totals[kBins];            // counts of the row
+  __shared__ __align__(16) unsigned hist[2][kBins];           // counts of this CTA; low and high words of the bins' sums
+  __shared__ __align__(16) unsigned totals[kBins];            // counts of the row
   __shared__ __align__(16) u64 bins[kBins];     // sums over the cluster of the bins this CTA looks after
   __shared__ double powers[32];                 // 2^(i / 32)
   __shared__ unsigned kmax_all, list_n, list_at, list_base;
-  __shared__ u64 posted[4][kMaxCluster];        // a value from every CTA of the cluster, four exchanges deep
+  __shared__ u64 posted[4][3][kMaxCluster];     // up to three values of every CTA, four exchanges deep
   __shared__ u64 result[2][2];
-  __shared__ u64 warp_part[kWarps];
+  __shared__ u64 warp_part[3][kWarps];
   __shared__ u64 carry;
   Words4* slice = reinterpret_cast<Words4*>(sample_smem);  // [per_cta] if kCached
   u64* units    = reinterpret_cast<u64*>(slice + (kCached ? a.per_cta : 0));  // sums of 32 vectors each, in order
   const unsigned rank = distill::cluster_rank();
   const unsigned size = distill::cluster_size();
   const int tid = int(threadIdx.x), warp = tid >> 5, lane = tid & 31;
-  for (int i = tid; i < kBins; i += kThreads)
-    hist[0][i] = totals[i] = 0;
-  if (tid < 32) powers[tid] = exp2(double(tid) * 0.03125);
-  if (tid == 0) kmax_all = list_n = list_at = 0;
-  __syncthreads();
-  distill::cluster_arrive();
   grid_dep_sync();
-
   const int64_t row = int64_t(blockIdx.x) / size;
   const T* z        = a.logits + row * a.ldl;
   const RowPart<T> part(z, a.vocab, int(rank) * a.per_cta, a.per_cta);
+  if constexpr (kCached) {  // every thread its own vectors, all of them under way at once
+    for (int j = tid; j < part.n; j += kThreads) {
+      if (part.whole(j))
+        distill::copy_async16(slice + j, part.at + j * VE);
+      else
+        slice[j] = part.load_edge(j);
+    }
+    distill::copy_commit();
+  }
+  for (int i = tid; i < kBins / 4; i += kThreads)
+    reinterpret_cast<uint4*>(hist[0])[i] = reinterpret_cast<uint4*>(totals)[i] = make_uint4(0, 0, 0, 0);
+  if (tid < 32) powers[tid] = kPowers[tid];
+  if (tid == 0) kmax_all = list_n = list_at = 0;
+  __syncthreads();
+  distill::cluster_arrive();  // every CTA of the cluster has started and is set up
   const float temp   = a.temperature != nullptr ? a.temperature[row] : a.temperature_all;
   const int top_k    = a.top_k != nullptr ? a.top_k[row] : a.top_k_all;
   const float top_p  = a.top_p != nullptr ? a.top_p[row] : a.top_p_all;
   const float min_p  = a.min_p != nullptr ? a.min_p[row] : a.min_p_all;
   const float u      = a.uniform[row];
   const bool greedy  = !(temp > 0.0f);
-  const auto vec     = [&](int j) { return kCached ? slice[j] : part.load(j); };
+  const auto vec     = [&](int j) { return kCached ? slice[j] : K::pack(part.load(j)); };  // keys
   int exchanges      = 0;
 
-  // every CTA's v, known to all afterwards (four calls long)
+  // every CTA's values, known to all afterwards (four calls long)
+  auto post3 = [&](u64 v0, u64 v1, u64 v2) {
+    auto slot = posted[exchanges & 3];
+    ++exchanges;
+    if (tid < int(size)) {
+      cluster_store_u64(&slot[0][rank], unsigned(tid), v0);
+      cluster_store_u64(&slot[1][rank], unsigned(tid), v1);
+      cluster_store_u64(&slot[2][rank], unsigned(tid), v2);
+    }
+    cluster_sync();
+    return slot;
+  };
   auto post = [&](u64 v) {
-    u64* slot = posted[exchanges & 3];
+    u64* slot = posted[exchanges & 3][0];
     ++exchanges;
     if (tid < int(size)) cluster_store_u64(&slot[rank], unsigned(tid), v);
     cluster_sync();
@@ -230,12 +274,12 @@ sample_kernel(const Args<T> a)
   auto block_sum = [&](u64 v) {  // to all threads
     v = warp_sum_u64(v);
     __syncthreads();
-    if (lane == 0) warp_part[warp] = v;
+    if (lane == 0) warp_part[0][warp] = v;
     __syncthreads();
     u64 s = 0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w)
-      s += warp_part[w];
+      s += warp_part[0][w];
     return s;
   };
 
@@ -246,12 +290,13 @@ sample_kernel(const Args<T> a)
   const bool counted = by_k || by_p || by_min;
   constexpr int kLow = K::kBits - kDigitBits;  // bits behind the first digit
   unsigned kmax      = 0;
+  if constexpr (kCached) distill::copy_wait<0>();
   for (int j = tid; j < part.n; j += kThreads) {
-    const Words4 v = part.load(j);
+    const Words4 v = K::pack(kCached ? slice[j] : part.load(j));
     if (kCached) slice[j] = v;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      const unsigned key = K::of(v, e);
+      const unsigned key = K::at(v, e);
       kmax               = max(kmax, key);
       if (counted && key > K::kNegInf) atomicAdd(&hist[0][key >> kLow], 1u);
     }
@@ -281,17 +326,18 @@ sample_kernel(const Args<T> a)
     if (rank == 0 && tid == 0) write(-1, -INFINITY);
     return;
   }
-  const double zmax  = double(K::value(kmax));
-  const double slope = 1.4426950408889634 / double(temp);
   // 2^x by table and polynomial: x * 32 = n + r, 2^x = 2^(n / 32) 2^(r / 32), the second by its Taylor series to the
-  // fifth power (|r / 32| <= 1 / 64: 3e-15), the first from `powers` and an exponent (P. T. P. Tang, 1989)
+  // fifth power (|r / 32| <= 1 / 64: 3e-15), the first from `powers` and an exponent (P. T. P. Tang, 1989). What rounds
+  // to 0 is cut off at `low` (and NaN there is none); temperatures above 1e30 count as that.
+  const double zmax    = double(K::value(kmax));
+  const double slope   = 1.4426950408889634 / double(fminf(temp, 1e30f));
   const double slope32 = slope * 32.0;
   const int shift      = a.shift;
+  const bool infinite  = kmax == K::kZero + (K::kZero - K::kNegInf);  // a +inf logit: the others weigh nothing
+  const float low      = fmaxf(__double2float_rd(zmax - double(shift + 2) / slope), -FLT_MAX);
   const auto weight    = [&](unsigned key) -> u64 {
-    if (key == kmax) return u64(1) << shift;
-    const double y = (double(K::value(key)) - zmax) * slope32;
-    if (!(y > -32.0 * double(kMaxShift + 2))) return 0;  // (and -inf * 0: a +inf logit at infinite temperature)
-    const double big = y + 6755399441055744.0;           // 1.5 * 2^52: the nearest integer in the low bits
+    const double y   = (double(fmaxf(K::value(key), low)) - zmax) * slope32;
+    const double big = y + 6755399441055744.0;  // 1.5 * 2^52: the nearest integer in the low bits
     const int n      = __double2loint(big);
     const double r   = (y - (big - 6755399441055744.0)) * (0.6931471805599453 / 32.0);
     double p         = fma(r, 1.0 / 120.0, 1.0 / 24.0);
@@ -301,7 +347,8 @@ sample_kernel(const Args<T> a)
     p                = fma(p, r, 1.0);
     const double w   = p * powers[n & 31];
     const double s   = __hiloint2double(__double2hiint(w) + (((n >> 5) + shift) << 20), __double2loint(w));
-    return u64(__double_as_longlong(s + 4503599627370496.0)) & 0xfffffffffffffull;  // 2^52: rounds to an integer
+    const u64 whole  = u64(__double_as_longlong(s + 4503599627370496.0)) & 0xfffffffffffffull;  // 2^52: to an integer
+    return !infinite ? whole : (key == kmax ? u64(1) << shift : 0);
   };
 
   // kept: key > tau, or key == tau and token <= last
@@ -318,18 +365,18 @@ sample_kernel(const Args<T> a)
         const Words4 v = vec(j0 + lane);
 #pragma unroll
         for (int e = 0; e < VE; ++e)
-          s += value(K::of(v, e), part.first + (j0 + lane) * VE + e);
+          s += value(K::at(v, e), part.first + (j0 + lane) * VE + e);
       }
       s = warp_sum_u64(s);
       if (lane == 0) units[j0 / 32] = s;
       own += s;
     }
     __syncthreads();
-    if (lane == 0) warp_part[warp] = own;
+    if (lane == 0) warp_part[0][warp] = own;
     __syncthreads();
     own = 0;
     for (int w = 0; w < kWarps; ++w)
-      own += warp_part[w];
+      own += warp_part[0][w];
     const u64* all = post(own);
     u64 total = 0, ahead = 0;
     for (unsigned r = 0; r < size; ++r) {
@@ -359,13 +406,13 @@ sample_kernel(const Args<T> a)
       run = __shfl_sync(distill::kFull, incl, 31);
     }
     const int j = at * 32 + lane;
-    Words4 v    = distill::minus_inf<T>();
+    Words4 v    = K::pack(distill::minus_inf<T>());
     u64 s       = 0;
     if (j < part.n) {
       v = vec(j);
 #pragma unroll
       for (int e = 0; e < VE; ++e)
-        s += value(K::of(v, e), part.first + j * VE + e);
+        s += value(K::at(v, e), part.first + j * VE + e);
     }
     const u64 incl      = run + warp_scan_u64(s);
     const unsigned over = __ballot_sync(distill::kFull, incl > target);
@@ -376,10 +423,10 @@ sample_kernel(const Args<T> a)
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       const int t = part.first + j * VE + e;
-      upto += value(K::of(v, e), t);
+      upto += value(K::at(v, e), t);
       if (token < 0 && upto > target) {
         token = t;
-        found = K::of(v, e);
+        found = K::at(v, e);
       }
     }
     *key = __shfl_sync(distill::kFull, found, l);
@@ -406,7 +453,7 @@ sample_kernel(const Args<T> a)
         const Words4 v = vec(j);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
-          const unsigned key = K::of(v, e);
+          const unsigned key = K::at(v, e);
           if ((left == K::kBits || (key >> left) == prefix) && kept(key, part.first + j * VE + e)) {
             const unsigned d = (key >> shift) & unsigned(n - 1);
             if constexpr (kCount) {
@@ -515,23 +562,48 @@ sample_kernel(const Args<T> a)
   // w >= min_p, as a bound on the key
   const double mp     = min_p < 1.0f ? double(min_p) : 1.0;
   const unsigned kmin = !by_min ? 0u : (mp == 1.0 ? kmax : min(kmax, K::at_least(zmax + log2(mp) / slope)));
-  const auto tokens_from = [&](const unsigned* counts, unsigned bin) {
+  // tokens of the bins from `bin` up: of the row in the high word, of this CTA in the low one
+  const auto tokens_from = [&](unsigned bin) {
     u64 s = 0;
     for (int i = tid; i < kBins; i += kThreads)
-      s += unsigned(i) >= bin ? counts[i] : 0u;
+      if (unsigned(i) >= bin) s += (u64(totals[i]) << 32) | hist[0][i];
     return block_sum(s);
   };
+  // The largest bin from which up there are at least `goal` tokens (0: there are fewer in all).
+  const auto bin_of = [&](u64 goal) {
+    constexpr int kEach = kBins / kThreads;
+    const int top       = kBins - 1 - tid * kEach;
+    u64 s               = 0;
+#pragma unroll
+    for (int q = 0; q < kEach; ++q)
+      s += totals[top - q];
+    const u64 incl = warp_scan_u64(s);
+    __syncthreads();
+    if (lane == 31) warp_part[0][warp] = incl;
+    if (tid == 0) carry = 0;
+    __syncthreads();
+    u64 run = incl - s;
+    for (int w = 0; w < warp; ++w)
+      run += warp_part[0][w];
+    if (run < goal && goal <= run + s) {
+      int q = 0;
+      while ((run += totals[top - q]) < goal)
+        ++q;
+      carry = u64(top - q);
+    }
+    __syncthreads();
+    return unsigned(carry);
+  };
   // Draws from the tokens of the bins from `bin` up, all of whose n are collected in the first CTA. `whole`: the weight
-  // of all tokens that top-p is measured by, or 0: that of the first top_k and min-p leave.
-  auto draw_from_list = [&](unsigned bin, int n, u64 whole) {
-    const u64 own = tokens_from(hist[0], bin);
-    if (tid == 0) list_base = cluster_fetch_add_u32(&list_n, 0, unsigned(own));
+  // of all tokens that top-p is measured by, or 0: that of the first top_k and min-p leave. `own` of them are here.
+  auto draw_from_list = [&](unsigned bin, int n, unsigned own, u64 whole) {
+    if (tid == 0) list_base = cluster_fetch_add_u32(&list_n, 0, own);
     __syncthreads();
     for (int j = tid; j < part.n && own != 0; j += kThreads) {
       const Words4 v = vec(j);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const unsigned key = K::of(v, e);
+        const unsigned key = K::at(v, e);
         if (key > K::kNegInf && (key >> kLow) >= bin) {
           const unsigned token = unsigned(part.first + j * VE + e);
           // larger keys first, lower tokens first among equals
@@ -545,6 +617,21 @@ sample_kernel(const Args<T> a)
     u64* weights = reinterpret_cast<u64*>(&hist[0][0]);  // [kList]
     // falling order of list[0 .. n)
     const auto sort = [&](int count) {
+      if (count <= kShort) {  // a thread's place is the number of larger ones; no two are equal
+        __syncthreads();
+        const u64 mine = tid < count ? list[tid] : 0;
+        if (tid >= count && tid < (count + 1) / 2 * 2) list[tid] = 0;
+        __syncthreads();
+        int place = 0;
+        for (int i = 0; i < count; i += 2) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list + i);
+          place += (x.x > mine ? 1 : 0) + (x.y > mine ? 1 : 0);
+        }
+        __syncthreads();
+        if (tid < count) list[place] = mine;
+        __syncthreads();
+        return;
+      }
       int padded = 32;
       while (padded < count)
         padded *= 2;
@@ -579,12 +666,12 @@ sample_kernel(const Args<T> a)
       }
       const u64 incl = warp_scan_u64(s);
       __syncthreads();
-      if (lane == 31) warp_part[warp] = incl;
+      if (lane == 31) warp_part[0][warp] = incl;
       __syncthreads();
       u64 base = incl - s, sum = 0;
       for (int w = 0; w < kWarps; ++w) {
-        base += w < warp ? warp_part[w] : 0;
-        sum += warp_part[w];
+        base += w < warp ? warp_part[0][w] : 0;
+        sum += warp_part[0][w];
       }
 #pragma unroll
       for (int q = 0; q < kEach; ++q)
@@ -642,61 +729,55 @@ sample_kernel(const Args<T> a)
         done(int(0xffffffffu - unsigned(list[i] >> 32)), unsigned(list[i]));
   };
   if (by_k || by_min) {
-    unsigned bin = kmin >> kLow;
-    if (by_k) {  // the bin at which the counts, from the largest keys down, reach top_k
-      constexpr int kEach = kBins / kThreads;
-      const int top       = kBins - 1 - tid * kEach;
-      u64 s               = 0;
-#pragma unroll
-      for (int q = 0; q < kEach; ++q)
-        s += totals[top - q];
-      const u64 incl = warp_scan_u64(s);
-      if (lane == 31) warp_part[warp] = incl;
-      if (tid == 0) carry = 0;
-      __syncthreads();
-      u64 run = incl - s;
-      for (int w = 0; w < warp; ++w)
-        run += warp_part[w];
-      if (run < u64(top_k) && u64(top_k) <= run + s) {
-        int q = 0;
-        while ((run += totals[top - q]) < u64(top_k))
-          ++q;
-        carry = u64(top - q);
-      }
-      __syncthreads();
-      bin = max(bin, unsigned(carry));
-    }
-    const u64 n = tokens_from(totals, bin);
-    if (n <= kList) {
-      draw_from_list(bin, int(n), 0);
+    const unsigned bin = max(kmin >> kLow, by_k ? bin_of(u64(top_k)) : 0u);
+    const u64 n        = tokens_from(bin);
+    if ((n >> 32) <= kList) {
+      draw_from_list(bin, int(n >> 32), unsigned(n), 0);
       return;
     }
   } else if (by_p) {
-    unsigned bin;
-    u64 above, whole;
-    const auto target_of = [&](u64 sum) {
-      const double t = ceil(double(top_p) * double(sum));
-      const u64 goal = t >= 1.0 ? u64(t) : 1;
-      return goal < sum ? goal : sum;
-    };
-    (void)select(std::false_type{}, weight, target_of, 1, &bin, &above, &whole);
-    const u64 n = tokens_from(totals, bin);
-    if (n <= kList) {
-      // (the histogram has been used for weights: this CTA's counts again)
-      __syncthreads();
-      for (int i = tid; i < kBins; i += kThreads)
-        hist[0][i] = 0;
-      __syncthreads();
-      for (int j = tid; j < part.n; j += kThreads) {
-        const Words4 v = vec(j);
+    // beginnings of at most kShort and kList tokens, and their weights
+    const unsigned bin1 = bin_of(kShort + 1) + 1, bin2 = bin_of(kList + 1) + 1;
+    u64 s0 = 0, s1 = 0, s2 = 0;
+    for (int j = tid; j < part.n; j += kThreads) {
+      const Words4 v = vec(j);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) {
-          const unsigned key = K::of(v, e);
-          if (key > K::kNegInf && (key >> kLow) >= bin) atomicAdd(&hist[0][key >> kLow], 1u);
-        }
+      for (int e = 0; e < VE; ++e) {
+        const unsigned key = K::at(v, e);
+        const u64 w        = key > K::kNegInf ? weight(key) : 0;
+        s0 += w;
+        s1 += (key >> kLow) >= bin1 ? w : 0;
+        s2 += (key >> kLow) >= bin2 ? w : 0;
       }
-      __syncthreads();
-      draw_from_list(bin, int(n), whole);
+    }
+    s0 = warp_sum_u64(s0);
+    s1 = warp_sum_u64(s1);
+    s2 = warp_sum_u64(s2);
+    __syncthreads();
+    if (lane == 0) {
+      warp_part[0][warp] = s0;
+      warp_part[1][warp] = s1;
+      warp_part[2][warp] = s2;
+    }
+    __syncthreads();
+    s0 = s1 = s2 = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      s0 += warp_part[0][w];
+      s1 += warp_part[1][w];
+      s2 += warp_part[2][w];
+    }
+    const auto all = post3(s0, s1, s2);
+    s0 = s1 = s2 = 0;
+    for (unsigned r = 0; r < size; ++r) {
+      s0 += all[0][r];
+      s1 += all[1][r];
+      s2 += all[2][r];
+    }
+    const double goal = double(top_p) * double(s0);
+    if (double(s2) >= goal && s2 > 0) {
+      const unsigned bin = double(s1) >= goal && s1 > 0 ? bin1 : bin2;
+      const u64 n        = tokens_from(bin);
+      draw_from_list(bin, int(n >> 32), unsigned(n), s0);
       return;
     }
   }
