@@ -10,13 +10,18 @@
 // the whole, so weights are computed in fp64 and summed as INTEGERS of 2^-shift, shift = 62 - ceil(log2 vocab) but at
 // most kMaxShift (45 bits for 131072 tokens): exact, the same whatever the order, the split of the row or the number of rows of the call.
 //
-// A cluster of CTAs takes a row, every CTA a part, which it keeps in shared memory. The logits' bits, made to rise with
-// their value, are counted by their first kDigitBits as soon as the row has come in, and the counts bound the beginning
-// of the order that can be kept: by top_k, by the bin of the lowest logit that min_p admits, or, for a top-p alone, by
-// taking a beginning of at most kShort or kList tokens and looking whether its weight is enough. It is collected in the
-// first CTA, sorted, and the rest happens there; the others are done. Longer beginnings (a flat distribution, a large k)
-// are narrowed by radix selection, a digit at a time, by counts or weights summed over the cluster through distributed
-// shared memory, and drawn from in place.
+// A cluster of CTAs takes a row, every CTA a part, which it keeps in shared memory. What is kept is nearly always a short
+// beginning of the order, and the work is in not touching the rest more than once or twice, two elements at a time:
+//   - every thread takes the maximum of its elements. The maxima are counted over the cluster by their keys (the logits'
+//     bits, made to rise with their value), in bins of 1/128 octave from the largest down: where n maxima lie at or
+//     above a bound there are at least n such elements, so the bin of the top_k-th maximum bounds the first top_k
+//     elements from below, and min_p is a bound by itself. For a top-p alone, beginnings that hold kShort / 2 and
+//     kList / 2 maxima are tried: whether their weight is enough is seen when the row's whole weight is summed, which a
+//     top-p needs anyway.
+//   - the elements above the bound, if they are at most kList, are collected in the first CTA, sorted, and the rest
+//     happens there; the other CTAs are done.
+// Longer beginnings (a flat distribution, a large k) are narrowed by radix selection over all elements, a digit at a
+// time, by counts or weights summed over the cluster through distributed shared memory, and drawn from in place.
 #pragma once
 
 #include "launch.cuh"
@@ -102,6 +107,61 @@ struct KeyOf {
       T x;
       memcpy(&x, &b, 2);
       return FloatIo<T>::up(x);
+    }
+  }
+  // bits of element e
+  B2R_DI static unsigned bits_at(const Words4& v, int e) { return at(v, e); }
+  // element e as fp32 (NaN as it is)
+  B2R_DI static float float_at(const Words4& v, int e)
+  {
+    const float2 f = up_pair<T>(v, e / 2);
+    return (e & 1) ? f.y : f.x;
+  }
+  // the larger ones of two words' elements (NaN loses)
+  B2R_DI static uint32_t larger(uint32_t a, uint32_t b)
+  {
+    if constexpr (kBits == 32) {
+      return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+    } else {
+      using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      Pair x, y;
+      memcpy(&x, &a, 4);
+      memcpy(&y, &b, 4);
+      x = __hmax2(x, y);
+      memcpy(&a, &x, 4);
+      return a;
+    }
+  }
+  B2R_DI static Words4 larger(const Words4& a, const Words4& b)
+  {
+    Words4 r;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      r.w[q] = larger(a.w[q], b.w[q]);
+    return r;
+  }
+  // the largest element as fp32 (NaN only if all are)
+  B2R_DI static float largest(const Words4& v)
+  {
+    Words<1> m;
+    m.w[0] = larger(larger(v.w[0], v.w[1]), larger(v.w[2], v.w[3]));
+    if constexpr (kBits == 32) {
+      return __uint_as_float(m.w[0]);
+    } else {
+      const float2 f = up_pair<T>(m, 0);
+      return fmaxf(f.x, f.y);
+    }
+  }
+  // key of a value that an element of T can have
+  B2R_DI static unsigned of_value(float x)
+  {
+    if constexpr (kBits == 32) {
+      return of_bits(__float_as_uint(x));
+    } else {
+      const T h = FloatIo<T>::down(x);
+      uint16_t b;
+      memcpy(&b, &h, 2);
+      return of_bits(b);
     }
   }
   // lowest key whose value is at least x
@@ -203,6 +263,8 @@ B2R_DI void cluster_sync()
   distill::cluster_wait();
 }
 
+B2R_HDI constexpr int bins_of(int size) { return kBins / size > kList ? kBins / size : kList; }
+
 template <typename T, bool kCached>
 __global__ void __launch_bounds__(kThreads, 2)
 sample_kernel(const Args<T> a)
@@ -210,19 +272,20 @@ sample_kernel(const Args<T> a)
   constexpr int VE = Vec16Of<T>::value;
   using K          = Key<T>;
   extern __shared__ __align__(16) unsigned char sample_smem[];
-  __shared__ __align__(16) unsigned hist[2][kBins];           // counts of this CTA; low and high words of the bins' sums
-  __shared__ __align__(16) unsigned totals[kBins];            // counts of the row
-  __shared__ __align__(16) u64 bins[kBins];     // sums over the cluster of the bins this CTA looks after
+  __shared__ __align__(16) unsigned hist[2][kBins];  // counts of this CTA and of the row; words of the bins' sums
   __shared__ double powers[32];                 // 2^(i / 32)
-  __shared__ unsigned kmax_all, list_n, list_at, list_base;
-  __shared__ u64 posted[4][3][kMaxCluster];     // up to three values of every CTA, four exchanges deep
+  __shared__ unsigned kmax_all, list_at;
+  __shared__ u64 posted[4][4][kMaxCluster];     // up to four values of every CTA, four exchanges deep
   __shared__ u64 result[2][2];
-  __shared__ u64 warp_part[3][kWarps];
+  __shared__ u64 warp_part[4][kWarps];
   __shared__ u64 carry;
   Words4* slice = reinterpret_cast<Words4*>(sample_smem);  // [per_cta] if kCached
-  u64* units    = reinterpret_cast<u64*>(slice + (kCached ? a.per_cta : 0));  // sums of 32 vectors each, in order
   const unsigned rank = distill::cluster_rank();
   const unsigned size = distill::cluster_size();
+  // sums over the cluster of the bins this CTA looks after; the list
+  u64* bins        = reinterpret_cast<u64*>(slice + (kCached ? a.per_cta : 0));  // [bins_of(size)]
+  u64* units       = bins + bins_of(int(size));                                  // sums of 32 vectors each, in order
+  unsigned* totals = hist[1];
   const int tid = int(threadIdx.x), warp = tid >> 5, lane = tid & 31;
   grid_dep_sync();
   const int64_t row = int64_t(blockIdx.x) / size;
@@ -240,7 +303,7 @@ sample_kernel(const Args<T> a)
   for (int i = tid; i < kBins / 4; i += kThreads)
     reinterpret_cast<uint4*>(hist[0])[i] = reinterpret_cast<uint4*>(totals)[i] = make_uint4(0, 0, 0, 0);
   if (tid < 32) powers[tid] = kPowers[tid];
-  if (tid == 0) kmax_all = list_n = list_at = 0;
+  if (tid == 0) kmax_all = list_at = 0;
   __syncthreads();
   distill::cluster_arrive();  // every CTA of the cluster has started and is set up
   const float temp   = a.temperature != nullptr ? a.temperature[row] : a.temperature_all;
@@ -249,17 +312,25 @@ sample_kernel(const Args<T> a)
   const float min_p  = a.min_p != nullptr ? a.min_p[row] : a.min_p_all;
   const float u      = a.uniform[row];
   const bool greedy  = !(temp > 0.0f);
-  const auto vec     = [&](int j) { return kCached ? slice[j] : K::pack(part.load(j)); };  // keys
+  const auto raw     = [&](int j) { return kCached ? slice[j] : part.load(j); };
+  const auto vec     = [&](int j) { return K::pack(raw(j)); };  // keys
   int exchanges      = 0;
 
+  auto write = [&](int64_t token, float logprob) {  // by one thread of the cluster
+    if (a.out64)
+      static_cast<long long*>(a.out)[row] = token;
+    else
+      static_cast<int*>(a.out)[row] = int(token);
+    if (a.logprobs != nullptr) a.logprobs[row] = logprob;
+  };
   // every CTA's values, known to all afterwards (four calls long)
-  auto post3 = [&](u64 v0, u64 v1, u64 v2) {
+  auto post4 = [&](const u64 (&v)[4]) {
     auto slot = posted[exchanges & 3];
     ++exchanges;
     if (tid < int(size)) {
-      cluster_store_u64(&slot[0][rank], unsigned(tid), v0);
-      cluster_store_u64(&slot[1][rank], unsigned(tid), v1);
-      cluster_store_u64(&slot[2][rank], unsigned(tid), v2);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        cluster_store_u64(&slot[q][rank], unsigned(tid), v[q]);
     }
     cluster_sync();
     return slot;
@@ -283,47 +354,49 @@ sample_kernel(const Args<T> a)
     return s;
   };
 
-  // the row, its largest key, and (where anything is to be left out) the counts by the first digit
-  const bool by_k    = !greedy && top_k > 0 && top_k < a.vocab;
-  const bool by_p    = !greedy && top_p < 1.0f;
-  const bool by_min  = !greedy && min_p > 0.0f;
-  const bool counted = by_k || by_p || by_min;
-  constexpr int kLow = K::kBits - kDigitBits;  // bits behind the first digit
-  unsigned kmax      = 0;
+  // the row; every thread's largest element, and the row's
+  const bool by_k   = !greedy && top_k > 0 && top_k < a.vocab;
+  const bool by_p   = !greedy && top_p < 1.0f;
+  const bool by_min = !greedy && min_p > 0.0f;
+  Words4 mine_max    = distill::minus_inf<T>();
   if constexpr (kCached) distill::copy_wait<0>();
-  for (int j = tid; j < part.n; j += kThreads) {
-    const Words4 v = K::pack(kCached ? slice[j] : part.load(j));
-    if (kCached) slice[j] = v;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-      const unsigned key = K::at(v, e);
-      kmax               = max(kmax, key);
-      if (counted && key > K::kNegInf) atomicAdd(&hist[0][key >> kLow], 1u);
-    }
-  }
+  for (int j = tid; j < part.n; j += kThreads)
+    mine_max = K::larger(mine_max, raw(j));
+  unsigned kmax = K::of_value(K::largest(mine_max));
+  const unsigned own_max = kmax;
   kmax = __reduce_max_sync(distill::kFull, kmax);
-  __syncthreads();
   distill::cluster_wait();
   if (lane < int(size)) cluster_max_u32(&kmax_all, unsigned(lane), kmax);
-  if (counted) {
-    for (int i = tid; i < kBins; i += kThreads) {
-      const unsigned n = hist[0][i];
-      if (n != 0)
-        for (unsigned r = 0; r < size; ++r)
-          cluster_add_u32(&totals[i], r, n);
-    }
-  }
   cluster_sync();
   kmax = kmax_all;
-  auto write = [&](int64_t token, float logprob) {  // by one thread of the cluster
-    if (a.out64)
-      static_cast<long long*>(a.out)[row] = token;
-    else
-      static_cast<int*>(a.out)[row] = int(token);
-    if (a.logprobs != nullptr) a.logprobs[row] = logprob;
-  };
   if (kmax <= K::kNegInf) {  // nothing to draw from
     if (rank == 0 && tid == 0) write(-1, -INFINITY);
+    return;
+  }
+  // f(vector, its first token) for the vectors that hold an element of at least `bound`
+  const auto vectors_from = [&](float bound, auto f) {
+    for (int j = tid; j < part.n; j += kThreads) {
+      const Words4 v = raw(j);
+      if (K::largest(v) >= bound) f(v, part.first + j * VE);
+    }
+  };
+  if (greedy) {  // the lowest token of those with the largest key
+    const float top = K::value(kmax);
+    unsigned token0 = 0xffffffffu;
+    vectors_from(top, [&](const Words4& v, int token) {
+#pragma unroll
+      for (int e = VE - 1; e >= 0; --e)
+        if (K::float_at(v, e) == top) token0 = min(token0, unsigned(token + e));
+    });
+    token0 = __reduce_min_sync(distill::kFull, token0);
+    if (lane == 0) warp_part[0][warp] = token0;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w)
+      token0 = min(token0, unsigned(warp_part[0][w]));
+    const u64* all = post(token0);
+    for (unsigned r = 0; r < size; ++r)
+      token0 = min(token0, unsigned(all[r]));
+    if (rank == 0 && tid == 0) write(int64_t(token0), 0.0f);
     return;
   }
   // 2^x by table and polynomial: x * 32 = n + r, 2^x = 2^(n / 32) 2^(r / 32), the second by its Taylor series to the
@@ -333,10 +406,15 @@ sample_kernel(const Args<T> a)
   const double slope   = 1.4426950408889634 / double(fminf(temp, 1e30f));
   const double slope32 = slope * 32.0;
   const int shift      = a.shift;
-  const bool infinite  = kmax == K::kZero + (K::kZero - K::kNegInf);  // a +inf logit: the others weigh nothing
-  const float low      = fmaxf(__double2float_rd(zmax - double(shift + 2) / slope), -FLT_MAX);
-  const auto weight    = [&](unsigned key) -> u64 {
-    const double y   = (double(fmaxf(K::value(key), low)) - zmax) * slope32;
+  const float top      = K::value(kmax);
+  const float cut      = __double2float_rd(zmax - double(shift + 2) / slope);
+  // no other logit counts: a +inf one, or floats further apart than the cut
+  const bool sharp     = top == INFINITY || cut >= nextafterf(top, -INFINITY);
+  const bool bottom    = cut < -FLT_MAX;  // logits near the lowest value: -inf has to be told from what counts
+  const float low      = fmaxf(cut, -FLT_MAX);
+  const bool special   = sharp || bottom;
+  const auto weight_of = [&](float z) -> u64 {
+    const double y   = (double(fmaxf(z, low)) - zmax) * slope32;
     const double big = y + 6755399441055744.0;  // 1.5 * 2^52: the nearest integer in the low bits
     const int n      = __double2loint(big);
     const double r   = (y - (big - 6755399441055744.0)) * (0.6931471805599453 / 32.0);
@@ -348,24 +426,26 @@ sample_kernel(const Args<T> a)
     const double w   = p * powers[n & 31];
     const double s   = __hiloint2double(__double2hiint(w) + (((n >> 5) + shift) << 20), __double2loint(w));
     const u64 whole  = u64(__double_as_longlong(s + 4503599627370496.0)) & 0xfffffffffffffull;  // 2^52: to an integer
-    return !infinite ? whole : (key == kmax ? u64(1) << shift : 0);
+    if (!special) return whole;
+    return sharp ? (z == top ? u64(1) << shift : 0) : (z >= -FLT_MAX ? whole : 0);
   };
+  const auto weight = [&](unsigned key) { return weight_of(K::value(key)); };
 
   // kept: key > tau, or key == tau and token <= last
   unsigned tau = K::kNegInf + 1;
   int last     = 0x7fffffff;
   const auto kept = [&](unsigned key, int token) { return key > tau || (key == tau && token <= last); };
 
-  // Sums of value(key, token) over runs of 32 vectors; *before: of the CTAs ahead of this one. Returns the whole sum.
+  // Sums of value(vector, element, token) over runs of 32 vectors; *before: of the CTAs ahead of this one. Returns the whole sum.
   auto sum_in_order = [&](auto value, u64* before, u64* mine) {
     u64 own = 0;
     for (int j0 = warp * 32; j0 < part.n; j0 += kThreads) {
       u64 s = 0;
       if (j0 + lane < part.n) {
-        const Words4 v = vec(j0 + lane);
+        const Words4 v = raw(j0 + lane);
 #pragma unroll
         for (int e = 0; e < VE; ++e)
-          s += value(K::at(v, e), part.first + (j0 + lane) * VE + e);
+          s += value(v, e, part.first + (j0 + lane) * VE + e);
       }
       s = warp_sum_u64(s);
       if (lane == 0) units[j0 / 32] = s;
@@ -406,13 +486,13 @@ sample_kernel(const Args<T> a)
       run = __shfl_sync(distill::kFull, incl, 31);
     }
     const int j = at * 32 + lane;
-    Words4 v    = K::pack(distill::minus_inf<T>());
+    Words4 v    = distill::minus_inf<T>();
     u64 s       = 0;
     if (j < part.n) {
-      v = vec(j);
+      v = raw(j);
 #pragma unroll
       for (int e = 0; e < VE; ++e)
-        s += value(K::at(v, e), part.first + j * VE + e);
+        s += value(v, e, part.first + j * VE + e);
     }
     const u64 incl      = run + warp_scan_u64(s);
     const unsigned over = __ballot_sync(distill::kFull, incl > target);
@@ -423,10 +503,10 @@ sample_kernel(const Args<T> a)
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       const int t = part.first + j * VE + e;
-      upto += value(K::at(v, e), t);
+      upto += value(v, e, t);
       if (token < 0 && upto > target) {
         token = t;
-        found = K::at(v, e);
+        found = K::of_bits(K::bits_at(v, e));
       }
     }
     *key = __shfl_sync(distill::kFull, found, l);
@@ -527,7 +607,9 @@ sample_kernel(const Args<T> a)
   };
   // the token of the `nth` (from 1) kept element whose key is tau, as a limit for all CTAs
   auto limit_ties = [&](u64 nth) {
-    const auto is_tie = [&](unsigned key, int token) -> u64 { return key == tau && token <= last ? 1 : 0; };
+    const auto is_tie = [&](const Words4& v, int e, int token) -> u64 {
+      return K::of_bits(K::bits_at(v, e)) == tau && token <= last ? 1 : 0;
+    };
     u64 before, mine;
     const u64 total = sum_in_order(is_tie, &before, &mine);
     if (nth >= total) return;  // all of them
@@ -546,110 +628,154 @@ sample_kernel(const Args<T> a)
       if (all[r] != 0) last = int(all[r]) - 1;
   };
 
-  if (greedy) {
-    tau = kmax;
-    const auto is_max = [&](unsigned key, int) -> u64 { return key == kmax ? 1 : 0; };
-    u64 before, mine;
-    (void)sum_in_order(is_max, &before, &mine);
-    if (before == 0 && mine > 0 && warp == 0) {
-      unsigned key;
-      const int token = locate(is_max, 0, &key);
-      if (lane == 0) write(token, 0.0f);
-    }
-    return;
-  }
   // The lowest bin of the first digit that can hold kept tokens, and the number of tokens from it up.
   // w >= min_p, as a bound on the key
   const double mp     = min_p < 1.0f ? double(min_p) : 1.0;
   const unsigned kmin = !by_min ? 0u : (mp == 1.0 ? kmax : min(kmax, K::at_least(zmax + log2(mp) / slope)));
-  // tokens of the bins from `bin` up: of the row in the high word, of this CTA in the low one
-  const auto tokens_from = [&](unsigned bin) {
-    u64 s = 0;
-    for (int i = tid; i < kBins; i += kThreads)
-      if (unsigned(i) >= bin) s += (u64(totals[i]) << 32) | hist[0][i];
-    return block_sum(s);
+  // elements of at least `bound` in this CTA
+  const auto count_from = [&](float bound) {
+    u64 n = 0;
+    vectors_from(bound, [&](const Words4& v, int) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        n += K::float_at(v, e) >= bound ? 1 : 0;
+    });
+    return block_sum(n);
   };
-  // The largest bin from which up there are at least `goal` tokens (0: there are fewer in all).
-  const auto bin_of = [&](u64 goal) {
+  // Threads' maxima by their distance from the largest key, in bins of 2^kFine keys (a 128th of an octave; the last bin
+  // holds all that lie further down).
+  constexpr int kFine = K::kBits == 32 ? 16 : (std::is_same<T, __half>::value ? 3 : 0);
+  if (by_k || (by_p && !by_min)) {
+    if (own_max > K::kNegInf) atomicAdd(&hist[0][min((kmax - own_max) >> kFine, unsigned(kBins - 1))], 1u);
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kThreads) {
+      const unsigned n = hist[0][i];
+      if (n != 0)
+        for (unsigned r = 0; r < size; ++r)
+          cluster_add_u32(&totals[i], r, n);
+    }
+    cluster_sync();
+  }
+  const float lowest = K::value(K::kNegInf + 1);
+  // A bound at or above which there are at least `goal` threads' maxima (the lowest value: there are fewer in all).
+  const auto bound_of = [&](u64 goal) {
     constexpr int kEach = kBins / kThreads;
-    const int top       = kBins - 1 - tid * kEach;
     u64 s               = 0;
 #pragma unroll
     for (int q = 0; q < kEach; ++q)
-      s += totals[top - q];
+      s += totals[tid * kEach + q];
     const u64 incl = warp_scan_u64(s);
     __syncthreads();
     if (lane == 31) warp_part[0][warp] = incl;
-    if (tid == 0) carry = 0;
+    if (tid == 0) carry = kBins - 1;
     __syncthreads();
     u64 run = incl - s;
     for (int w = 0; w < warp; ++w)
       run += warp_part[0][w];
     if (run < goal && goal <= run + s) {
       int q = 0;
-      while ((run += totals[top - q]) < goal)
+      while ((run += totals[tid * kEach + q]) < goal)
         ++q;
-      carry = u64(top - q);
+      carry = u64(tid * kEach + q);
     }
     __syncthreads();
-    return unsigned(carry);
+    const unsigned down = (unsigned(carry) + 1) << kFine;  // the bin's lowest key is kmax - down + 1
+    const bool last_bin = carry == kBins - 1;
+    return last_bin || kmax < K::kNegInf + down ? lowest : K::value(kmax - down + 1);
   };
-  // Draws from the tokens of the bins from `bin` up, all of whose n are collected in the first CTA. `whole`: the weight
-  // of all tokens that top-p is measured by, or 0: that of the first top_k and min-p leave. `own` of them are here.
-  auto draw_from_list = [&](unsigned bin, int n, unsigned own, u64 whole) {
-    if (tid == 0) list_base = cluster_fetch_add_u32(&list_n, 0, own);
-    __syncthreads();
-    for (int j = tid; j < part.n && own != 0; j += kThreads) {
-      const Words4 v = vec(j);
+  // Draws from the n elements of at least `bound`, collected in the first CTA; `base` of them are in the CTAs ahead.
+  // `whole`: the weight of all tokens that top-p is measured by, or 0: that of those top_k and min-p leave.
+  auto draw_from_list = [&](float bound, int n, int base, u64 whole) {
+    vectors_from(bound, [&](const Words4& v, int first) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const unsigned key = K::at(v, e);
-        if (key > K::kNegInf && (key >> kLow) >= bin) {
-          const unsigned token = unsigned(part.first + j * VE + e);
+        if (K::float_at(v, e) >= bound) {
           // larger keys first, lower tokens first among equals
-          cluster_store_u64(&bins[list_base + atomicAdd(&list_at, 1u)], 0, (u64(key) << 32) | (0xffffffffu - token));
+          cluster_store_u64(&bins[base + int(atomicAdd(&list_at, 1u))], 0,
+                            (u64(K::of_bits(K::bits_at(v, e))) << 32) | (0xffffffffu - unsigned(first + e)));
         }
       }
-    }
+    });
     cluster_sync();
     if (rank != 0) return;
     u64* list    = bins;
     u64* weights = reinterpret_cast<u64*>(&hist[0][0]);  // [kList]
     // falling order of list[0 .. n)
     const auto sort = [&](int count) {
-      if (count <= kShort) {  // a thread's place is the number of larger ones; no two are equal
+      if (count <= kShort) {  // the place of a token is the number of larger ones; no two are equal
         __syncthreads();
-        const u64 mine = tid < count ? list[tid] : 0;
-        if (tid >= count && tid < (count + 1) / 2 * 2) list[tid] = 0;
-        __syncthreads();
-        int place = 0;
-        for (int i = 0; i < count; i += 2) {
-          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list + i);
-          place += (x.x > mine ? 1 : 0) + (x.y > mine ? 1 : 0);
+        u64 mine[kShort / kThreads];
+        int place[kShort / kThreads] = {};
+#pragma unroll
+        for (int q = 0; q < kShort / kThreads; ++q) {
+          const int i = tid + q * kThreads;
+          mine[q]     = i < count ? list[i] : 0;
+          if (i == count && (count & 1)) list[i] = 0;
         }
         __syncthreads();
-        if (tid < count) list[place] = mine;
+        for (int i = 0; i < count; i += 2) {
+          const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list + i);
+#pragma unroll
+          for (int q = 0; q < kShort / kThreads; ++q)
+            place[q] += (x.x > mine[q] ? 1 : 0) + (x.y > mine[q] ? 1 : 0);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < kShort / kThreads; ++q)
+          if (tid + q * kThreads < count) list[place[q]] = mine[q];
         __syncthreads();
         return;
       }
-      int padded = 32;
-      while (padded < count)
-        padded *= 2;
-      for (int i = count + tid; i < padded; i += kThreads)
-        list[i] = 0;
-      for (int k = 2; k <= padded; k *= 2) {
+      // bitonic, four neighbours per thread: exchanges within a thread, within a warp, and through shared memory only
+      // at distances of 128 and more (10 of 66 steps)
+      static_assert(kList == 4 * kThreads, "four places per thread");
+      u64 v[4];
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        v[q] = tid * 4 + q < count ? list[tid * 4 + q] : 0;
+      const auto order = [](u64& x, u64& y, bool falling) {  // the larger one first if falling
+        const u64 hi = x > y ? x : y, lo = x > y ? y : x;
+        x = falling ? hi : lo;
+        y = falling ? lo : hi;
+      };
+#pragma unroll 1
+      for (int k = 2; k <= kList; k *= 2) {
+#pragma unroll 1
         for (int h = k / 2; h > 0; h /= 2) {
-          __syncthreads();
-          for (int i = tid; i < padded / 2; i += kThreads) {
-            const int lo = 2 * i - (i & (h - 1)), hi = lo + h;
-            const u64 x = list[lo], y = list[hi];
-            if ((x < y) == ((lo & k) == 0)) {
-              list[lo] = y;
-              list[hi] = x;
+          if (h >= 4) {
+            u64 o[4];
+            if (h >= 128) {
+              __syncthreads();
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                list[tid * 4 + q] = v[q];
+              __syncthreads();
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                o[q] = list[(tid * 4 ^ h) + q];
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                o[q] = __shfl_xor_sync(distill::kFull, v[q], h / 4);
             }
+            const bool larger = ((tid * 4 & h) == 0) == ((tid * 4 & k) == 0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              v[q] = (v[q] > o[q]) == larger ? v[q] : o[q];
+          } else if (h == 2) {
+            order(v[0], v[2], (tid * 4 & k) == 0);
+            order(v[1], v[3], (tid * 4 & k) == 0);
+          } else {
+            order(v[0], v[1], (tid * 4 & k) == 0);
+            order(v[2], v[3], k == 2 ? false : (tid * 4 & k) == 0);
           }
         }
       }
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        list[tid * 4 + q] = v[q];
       __syncthreads();
     };
     sort(n);
@@ -729,55 +855,68 @@ sample_kernel(const Args<T> a)
         done(int(0xffffffffu - unsigned(list[i] >> 32)), unsigned(list[i]));
   };
   if (by_k || by_min) {
-    const unsigned bin = max(kmin >> kLow, by_k ? bin_of(u64(top_k)) : 0u);
-    const u64 n        = tokens_from(bin);
-    if ((n >> 32) <= kList) {
-      draw_from_list(bin, int(n >> 32), unsigned(n), 0);
+    const float bound = fmaxf(by_min ? K::value(kmin) : lowest, by_k ? bound_of(u64(top_k)) : lowest);
+    const u64* all    = post(count_from(bound));
+    u64 n = 0, base = 0;
+    for (unsigned r = 0; r < size; ++r) {
+      n += all[r];
+      base += r < rank ? all[r] : 0;
+    }
+    if (n <= kList) {
+      draw_from_list(bound, int(n), int(base), 0);
       return;
     }
   } else if (by_p) {
-    // beginnings of at most kShort and kList tokens, and their weights
-    const unsigned bin1 = bin_of(kShort + 1) + 1, bin2 = bin_of(kList + 1) + 1;
-    u64 s0 = 0, s1 = 0, s2 = 0;
+    const float bound1 = bound_of(kShort / 2), bound2 = bound_of(kList / 2);
+    u64 s[4] = {};  // the whole weight, that of the two beginnings, their lengths
     for (int j = tid; j < part.n; j += kThreads) {
-      const Words4 v = vec(j);
+      const Words4 v = raw(j);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const unsigned key = K::at(v, e);
-        const u64 w        = key > K::kNegInf ? weight(key) : 0;
-        s0 += w;
-        s1 += (key >> kLow) >= bin1 ? w : 0;
-        s2 += (key >> kLow) >= bin2 ? w : 0;
+        const float x = K::float_at(v, e);
+        const u64 w   = weight_of(x);
+        s[0] += w;
+        if (x >= bound2) {
+          s[2] += w;
+          s[3] += u64(1) << 32;
+          if (x >= bound1) {
+            s[1] += w;
+            s[3] += 1;
+          }
+        }
       }
     }
-    s0 = warp_sum_u64(s0);
-    s1 = warp_sum_u64(s1);
-    s2 = warp_sum_u64(s2);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      s[q] = warp_sum_u64(s[q]);
     __syncthreads();
     if (lane == 0) {
-      warp_part[0][warp] = s0;
-      warp_part[1][warp] = s1;
-      warp_part[2][warp] = s2;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        warp_part[q][warp] = s[q];
     }
     __syncthreads();
-    s0 = s1 = s2 = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      s0 += warp_part[0][w];
-      s1 += warp_part[1][w];
-      s2 += warp_part[2][w];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s[q] = 0;
+      for (int w = 0; w < kWarps; ++w)
+        s[q] += warp_part[q][w];
     }
-    const auto all = post3(s0, s1, s2);
-    s0 = s1 = s2 = 0;
-    for (unsigned r = 0; r < size; ++r) {
-      s0 += all[0][r];
-      s1 += all[1][r];
-      s2 += all[2][r];
+    const auto all = post4(s);
+    u64 ahead      = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      s[q] = 0;
+      for (unsigned r = 0; r < size; ++r)
+        s[q] += all[q][r];
     }
-    const double goal = double(top_p) * double(s0);
-    if (double(s2) >= goal && s2 > 0) {
-      const unsigned bin = double(s1) >= goal && s1 > 0 ? bin1 : bin2;
-      const u64 n        = tokens_from(bin);
-      draw_from_list(bin, int(n >> 32), unsigned(n), s0);
+    for (unsigned r = 0; r < rank; ++r)
+      ahead += all[3][r];
+    const double goal = double(top_p) * double(s[0]);
+    const int n1 = int(unsigned(s[3])), n2 = int(s[3] >> 32);
+    const bool first = double(s[1]) >= goal && n1 <= kList;
+    if (first || (double(s[2]) >= goal && n2 <= kList)) {
+      draw_from_list(first ? bound1 : bound2, first ? n1 : n2, first ? int(unsigned(ahead)) : int(ahead >> 32), s[0]);
       return;
     }
   }
@@ -810,23 +949,33 @@ sample_kernel(const Args<T> a)
       limit_ties((target - above + w - 1) / w);
     }
   }
-  const auto kept_weight = [&](unsigned key, int token) -> u64 { return kept(key, token) ? weight(key) : 0; };
-  u64 before, mine;
-  const u64 total = sum_in_order(kept_weight, &before, &mine);
-  const double t  = double(u) * double(total);
-  u64 target      = t > 0.0 ? u64(t) : 0;
-  if (target >= total) target = total - 1;  // u of 1 (or more) takes the last kept token
-  if (before <= target && target < before + mine && warp == 0) {
-    unsigned key;
-    const int token = locate(kept_weight, target - before, &key);
-    if (lane == 0) write(token, float(log(double(weight(key)) / double(total))));
+  const auto draw_in_place = [&](auto value) {
+    u64 before, mine;
+    const u64 total = sum_in_order(value, &before, &mine);
+    const double t  = double(u) * double(total);
+    u64 target      = t > 0.0 ? u64(t) : 0;
+    if (target >= total) target = total - 1;  // u of 1 (or more) takes the last kept token
+    if (before <= target && target < before + mine && warp == 0) {
+      unsigned key;
+      const int token = locate(value, target - before, &key);
+      if (lane == 0) write(token, float(log(double(weight(key)) / double(total))));
+    }
+  };
+  if (by_k || by_min || by_p) {
+    draw_in_place([&](const Words4& v, int e, int token) -> u64 {
+      const unsigned key = K::of_bits(K::bits_at(v, e));
+      return kept(key, token) ? weight(key) : 0;
+    });
+  } else {  // (NaN and -inf weigh 0)
+    draw_in_place([&](const Words4& v, int e, int) -> u64 { return weight_of(K::float_at(v, e)); });
   }
 }
 
 // ---------------------------------------------------------------------------------------
-// Host side. The smallest cluster whose parts take at most 64 KB (three CTAs per SM), larger ones while there are
-// fewer than two CTAs per SM; parts of up to kMaxPartKb where eight CTAs are not enough, and beyond that rows are read
-// from memory in every pass.
+// Host side. The smallest cluster whose parts take at most 64 KB (two CTAs per SM; 256 rows of 131072 bf16 in parts of
+// 32 KB and CTAs of 256 threads, three or four per SM, took a tenth longer: more CTAs to a cluster), larger ones while
+// there are fewer than two CTAs per SM; parts of up to kMaxPartKb where eight CTAs are not enough, and beyond that rows
+// are read from memory in every pass.
 // ---------------------------------------------------------------------------------------
 template <typename T>
 inline cudaError_t launch_sample(Args<T> a, cudaStream_t stream)
@@ -845,7 +994,7 @@ inline cudaError_t launch_sample(Args<T> a, cudaStream_t stream)
     --a.shift;
   const bool cached  = int64_t(a.per_cta) * 16 <= int64_t(kMaxPartKb) * 1024;
   const size_t units = size_t(ceil_div(a.per_cta, 32)) * sizeof(u64);
-  const size_t smem  = (cached ? size_t(a.per_cta) * 16 : 0) + units;
+  const size_t smem  = (cached ? size_t(a.per_cta) * 16 : 0) + size_t(bins_of(size)) * sizeof(u64) + units;
   const int64_t max_rows = int64_t(0x7fffffff) / size;
   auto kern              = cached ? sample_kernel<T, true> : sample_kernel<T, false>;
   cudaError_t e          = ensure_dynamic_smem(kern, smem);

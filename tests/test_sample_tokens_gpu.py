@@ -117,6 +117,27 @@ def test_equal_logits(cuda, dtype, vocab, filters):
     check(few, uniform, **filters)
 
 
+@pytest.mark.parametrize("scale", [1e-6, 1e-2, 30.0, 1e4, 1e12, 1e30])
+@pytest.mark.parametrize("shift", [0.0, -5.0, 5.0])
+def test_flat_peaked_and_distant_logits(cuda, scale, shift):
+    """Distributions from flat to one token; logits so large that neighbouring floats are whole units apart."""
+    logits, uniform, gen = make(40, 6001, torch.float32, cuda, 31, scale=scale)
+    logits += shift * scale
+    check(logits, uniform, **mixed(40, gen, cuda))
+    check(logits, uniform)
+    check(logits, uniform, top_p=0.7)
+
+
+@pytest.mark.parametrize("k", [400, 511, 512, 513, 900, 1500, 2047, 2048, 2049, 5000])
+@pytest.mark.parametrize("top_p", [1.0, 0.9, 0.3])
+def test_long_lists(cuda, k, top_p):
+    """Beginnings of the order around the lengths at which the way of sorting and of drawing changes."""
+    logits, uniform, _ = make(30, 20011, torch.float32, cuda, k, scale=0.7)
+    check(logits, uniform, top_k=k, top_p=top_p)
+    few = (logits * 8).round() / 8  # many equal logits
+    check(few, uniform, top_k=k, top_p=top_p)
+
+
 def test_every_token_gets_its_share(cuda):
     """The same row for a fine grid of uniform numbers: a token is drawn for the grid points of its interval."""
     n, vocab = 20000, 50
