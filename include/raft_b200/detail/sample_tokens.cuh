@@ -43,7 +43,8 @@ constexpr int kDigitBits  = 11;
 constexpr int kBins       = 1 << kDigitBits;
 constexpr int kMaxPartKb  = 160;  // of a row in a CTA's shared memory
 constexpr int kList       = 2048;
-constexpr int kShort      = 512;  // sorted by counting, a token per thread
+constexpr int kShort      = 256;  // up to here a list is sorted by comparing all pairs
+constexpr int kScratch    = kList * 12;  // bytes of the row's place in shared memory at least: the sort of a list
 constexpr int kMaxShift   = 50;  // weights below 2^51, so that an addition rounds them to integers
 
 template <typename T>
@@ -65,6 +66,7 @@ struct Args {
   int vocab;
   int per_cta;  // vectors of a row per CTA
   int shift;    // weights are integers of 2^-shift
+  int row_bytes;  // of the row's place in shared memory
 };
 
 // An element as an unsigned number of its own width that rises with its value: half the range plus or minus the bits
@@ -283,7 +285,7 @@ sample_kernel(const Args<T> a)
   const unsigned rank = distill::cluster_rank();
   const unsigned size = distill::cluster_size();
   // sums over the cluster of the bins this CTA looks after; the list
-  u64* bins        = reinterpret_cast<u64*>(slice + (kCached ? a.per_cta : 0));  // [bins_of(size)]
+  u64* bins        = reinterpret_cast<u64*>(sample_smem + a.row_bytes);  // [bins_of(size)]
   u64* units       = bins + bins_of(int(size));                                  // sums of 32 vectors each, in order
   unsigned* totals = hist[1];
   const int tid = int(threadIdx.x), warp = tid >> 5, lane = tid & 31;
@@ -700,85 +702,88 @@ sample_kernel(const Args<T> a)
     if (rank != 0) return;
     u64* list    = bins;
     u64* weights = reinterpret_cast<u64*>(&hist[0][0]);  // [kList]
-    // falling order of list[0 .. n)
-    const auto sort = [&](int count) {
-      if (count <= kShort) {  // the place of a token is the number of larger ones; no two are equal
+    // Falling order of list[0 .. count), no two of which are equal. bin_of(x), below kList, never falls as x does.
+    const auto sort = [&](int count, auto bin_of) {
+      constexpr int kEach = kList / kThreads;
+      if (count <= kShort) {  // the place of a token is the number of larger ones
         __syncthreads();
-        u64 mine[kShort / kThreads];
-        int place[kShort / kThreads] = {};
-#pragma unroll
-        for (int q = 0; q < kShort / kThreads; ++q) {
-          const int i = tid + q * kThreads;
-          mine[q]     = i < count ? list[i] : 0;
-          if (i == count && (count & 1)) list[i] = 0;
-        }
+        const u64 mine = tid < count ? list[tid] : 0;
+        if (tid == count && (count & 1)) list[tid] = 0;
         __syncthreads();
+        int place = 0;
         for (int i = 0; i < count; i += 2) {
           const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(list + i);
-#pragma unroll
-          for (int q = 0; q < kShort / kThreads; ++q)
-            place[q] += (x.x > mine[q] ? 1 : 0) + (x.y > mine[q] ? 1 : 0);
+          place += (x.x > mine ? 1 : 0) + (x.y > mine ? 1 : 0);
         }
         __syncthreads();
-#pragma unroll
-        for (int q = 0; q < kShort / kThreads; ++q)
-          if (tid + q * kThreads < count) list[place[q]] = mine[q];
+        if (tid < count) list[place] = mine;
         __syncthreads();
         return;
       }
-      // bitonic, four neighbours per thread: exchanges within a thread, within a warp, and through shared memory only
-      // at distances of 128 and more (10 of 66 steps)
-      static_assert(kList == 4 * kThreads, "four places per thread");
-      u64 v[4];
+      // into bins, by counts; then every token looks for its place among those of its bin, nearly always a few (a
+      // sorting network over 2048 places takes 14 us, mostly shuffles; this 2)
+      u64* spread     = reinterpret_cast<u64*>(sample_smem);              // [kList]
+      unsigned* start = reinterpret_cast<unsigned*>(spread + kList);      // [kList]
+#pragma unroll
+      for (int q = 0; q < kEach; ++q)
+        start[tid + q * kThreads] = 0;
       __syncthreads();
+      u64 x[kEach];
+      unsigned bin[kEach], at[kEach];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        v[q] = tid * 4 + q < count ? list[tid * 4 + q] : 0;
-      const auto order = [](u64& x, u64& y, bool falling) {  // the larger one first if falling
-        const u64 hi = x > y ? x : y, lo = x > y ? y : x;
-        x = falling ? hi : lo;
-        y = falling ? lo : hi;
-      };
-#pragma unroll 1
-      for (int k = 2; k <= kList; k *= 2) {
-#pragma unroll 1
-        for (int h = k / 2; h > 0; h /= 2) {
-          if (h >= 4) {
-            u64 o[4];
-            if (h >= 128) {
-              __syncthreads();
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                list[tid * 4 + q] = v[q];
-              __syncthreads();
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                o[q] = list[(tid * 4 ^ h) + q];
-            } else {
-#pragma unroll
-              for (int q = 0; q < 4; ++q)
-                o[q] = __shfl_xor_sync(distill::kFull, v[q], h / 4);
-            }
-            const bool larger = ((tid * 4 & h) == 0) == ((tid * 4 & k) == 0);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              v[q] = (v[q] > o[q]) == larger ? v[q] : o[q];
-          } else if (h == 2) {
-            order(v[0], v[2], (tid * 4 & k) == 0);
-            order(v[1], v[3], (tid * 4 & k) == 0);
-          } else {
-            order(v[0], v[1], (tid * 4 & k) == 0);
-            order(v[2], v[3], k == 2 ? false : (tid * 4 & k) == 0);
-          }
+      for (int q = 0; q < kEach; ++q) {
+        const int i = tid + q * kThreads;
+        if (i < count) {
+          x[q]   = list[i];
+          bin[q] = bin_of(x[q]);
+          at[q]  = atomicAdd(&start[bin[q]], 1u);
         }
       }
       __syncthreads();
+      unsigned n_bin[kEach], sum = 0;
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        list[tid * 4 + q] = v[q];
+      for (int q = 0; q < kEach; ++q) {
+        n_bin[q] = sum;
+        sum += start[tid * kEach + q];
+      }
+      const u64 incl = warp_scan_u64(sum);
+      if (lane == 31) warp_part[0][warp] = incl;
+      __syncthreads();
+      u64 base = incl - sum;
+      for (int w = 0; w < warp; ++w)
+        base += warp_part[0][w];
+#pragma unroll
+      for (int q = 0; q < kEach; ++q)
+        start[tid * kEach + q] = unsigned(base) + n_bin[q];
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kEach; ++q)
+        if (tid + q * kThreads < count) spread[start[bin[q]] + at[q]] = x[q];
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kEach; ++q) {
+        if (tid + q * kThreads < count) {
+          const unsigned from = start[bin[q]];
+          const unsigned to   = bin[q] + 1 < unsigned(kList) ? start[bin[q] + 1] : unsigned(count);
+          unsigned place      = from;
+          for (unsigned i = from; i < to; ++i)
+            place += spread[i] > x[q] ? 1u : 0u;
+          list[place] = x[q];
+        }
+      }
       __syncthreads();
     };
-    sort(n);
+    // by value: even steps from the largest logit down to the bound
+    const float step_v = top > bound ? float(kList - 1) / (top - bound) : 0.0f;
+    const auto value_bin = [&](u64 x) {
+      const float z = K::value(unsigned(x >> 32));
+      const float d = z == top ? 0.0f : (top - z) * step_v;  // (0 * inf is NaN: the first bin)
+      return d > 0.0f ? min(unsigned(d), unsigned(kList - 1)) : 0u;
+    };
+    const auto token_bin = [&](u64 x) {
+      return unsigned(u64(0xffffffffu - unsigned(x >> 32)) * unsigned(kList) / unsigned(a.vocab));
+    };
+    sort(n, value_bin);
     int m = by_k && top_k < n ? top_k : n;
     // running weights of the first m that min-p leaves (from it on all are below): four places per thread
     constexpr int kEach = kList / kThreads;
@@ -848,7 +853,7 @@ sample_kernel(const Args<T> a)
     for (int i = tid; i < m; i += kThreads)
       list[i] = (list[i] << 32) | (list[i] >> 32);  // complements of tokens fall where tokens rise
     __syncthreads();
-    sort(m);
+    sort(m, token_bin);
     (void)running([&](int i) { return weight(unsigned(list[i])); });
     for (int i = tid; i < m; i += kThreads)
       if (weights[i] > target && (i == 0 || weights[i - 1] <= target))
@@ -994,7 +999,9 @@ inline cudaError_t launch_sample(Args<T> a, cudaStream_t stream)
     --a.shift;
   const bool cached  = int64_t(a.per_cta) * 16 <= int64_t(kMaxPartKb) * 1024;
   const size_t units = size_t(ceil_div(a.per_cta, 32)) * sizeof(u64);
-  const size_t smem  = (cached ? size_t(a.per_cta) * 16 : 0) + size_t(bins_of(size)) * sizeof(u64) + units;
+  const int64_t held = cached ? int64_t(a.per_cta) * 16 : 0;
+  a.row_bytes        = int(held > kScratch ? held : kScratch);
+  const size_t smem  = size_t(a.row_bytes) + size_t(bins_of(size)) * sizeof(u64) + units;
   const int64_t max_rows = int64_t(0x7fffffff) / size;
   auto kern              = cached ? sample_kernel<T, true> : sample_kernel<T, false>;
   cudaError_t e          = ensure_dynamic_smem(kern, smem);
