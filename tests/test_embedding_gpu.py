@@ -138,13 +138,15 @@ def test_empty(cuda, n, vocab, cols):
         assert torch.all(grad == 0)
 
 
-# counting ranks up to 8192 positions, radix passes above: one pass up to 511 tokens, two up to 2^18 - 1, three above
+# one launch up to 1024 positions; above, counting ranks up to 8192, then radix passes: one up to 511 tokens, two up to
+# 2^18 - 1, three above
 @pytest.mark.parametrize("in_dtype,out_dtype", [(torch.float32, torch.float32), (torch.float16, torch.float16),
                                                 (torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16),
                                                 (torch.bfloat16, torch.float32)])
 @pytest.mark.parametrize("n,vocab,cols", [(1, 1, 1), (1, 300, 8), (2, 2, 33), (100, 1000, 64), (1000, 50, 777),
                                           (4096, 32000, 24), (8192, 100, 16), (8193, 511, 8), (9001, 512, 40),
-                                          (20011, 50001, 72), (40000, 300000, 9), (3000, 20, 1032)])
+                                          (20011, 50001, 72), (40000, 300000, 9), (3000, 20, 1032), (1023, 5000, 520),
+                                          (1024, 130, 1032), (1025, 130, 1031), (2000, 131072, 8)])
 @pytest.mark.parametrize("kind", ["skew", "ends", "uniform"])
 def test_grad(cuda, in_dtype, out_dtype, n, vocab, cols, kind):
     gen = torch.Generator(device=cuda).manual_seed(n + cols)
@@ -155,7 +157,7 @@ def test_grad(cuda, in_dtype, out_dtype, n, vocab, cols, kind):
     assert_grad(got, g, tokens, vocab, 0.6)
 
 
-@pytest.mark.parametrize("n", [1, 15, 16, 17, 31, 32, 33, 1000, 5000, 20000])
+@pytest.mark.parametrize("n", [1, 15, 16, 17, 31, 32, 33, 1000, 1024, 1025, 5000, 20000])
 @pytest.mark.parametrize("kind", ["one", "none"])
 @pytest.mark.parametrize("cols", [8, 13, 2056])
 def test_grad_of_one_token_everywhere_or_none(cuda, n, kind, cols):
