@@ -31,7 +31,7 @@ namespace emb {
 // Lookup. A group of G lanes takes (row, segment of U * G vectors): U loads in flight per lane, neighbouring lanes on
 // neighbouring vectors. Memory bound; nothing to reuse but rows that several tokens name, which L2 holds. U is four
 // 16-byte vectors, sixteen narrow ones where rows lie off 16-byte boundaries (10007 x 1001 fp16:
-// 16.3 us, 22.0 with four). 65536 x 4096 bf16: 120 us, 9.0 TB/s of rows read and written (L2 serves the repeated rows)..
+// 16.3 us, 22.0 with four). 65536 x 4096 bf16: 120 us, 9.0 TB/s of rows read and written (L2 serves the repeated rows).
 // ---------------------------------------------------------------------------------------
 constexpr int kLookupThreads = 256;
 template <typename T, int V>
@@ -518,7 +518,7 @@ sum_rows_kernel(OutT* out, int64_t ldo, float* partial, const InT* g, int64_t ld
 // and the commonest one has the most pieces, so what counts is the time of one thread's chain: four columns at most to
 // a thread (shape is this kernel's own), the last run by a search of the tokens before any piece is loaded, and kFold
 // pieces asked for together: 23 us of the 285 of 65536 x 4096 bf16 into 131072 rows, 37 with eight columns to a thread
-and the tokens read beside the pieces; 9.6 of the 84 of 20011 x 777 f16 into 50001 rows, 45 with sum_rows_kernel's shape.
+// and the tokens read beside the pieces; 9.6 of the 84 of 20011 x 777 f16 into 50001 rows, 45 with sum_rows_kernel's shape.
 template <typename OutT, int V>
 __global__ void __launch_bounds__(kSumThreads)
 fold_rows_kernel(OutT* out, int64_t ldo, const float* partial, const unsigned* skey, int64_t n, int64_t n_cols,
