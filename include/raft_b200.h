@@ -281,7 +281,7 @@ B2R_API int b2r_embedding_lookup(void* out,
  * otherwise the sums are added to what the rows hold and rows that no token names are left alone. Tokens outside
  * [0, vocab) add nothing. Sums are fp32, rounded once; their order depends on the positions alone, so results
  * repeat bit for bit. grad_out of type `dtype`, grad_table of the same type or B2R_F32; they must not overlap.
- * `workspace`: b2r_embedding_grad_workspace_bytes() bytes (256-byte aligned), or NULL.
+ * `workspace`: b2r_embedding_grad_workspace_bytes() bytes (256-byte aligned; 0 bytes up to 1024 tokens), or NULL.
  */
 B2R_API int b2r_embedding_grad(void* grad_table,
                                int64_t ldg,
@@ -370,7 +370,8 @@ B2R_API int b2r_topk_distill_grad(void* grad,
  * row's token does not depend on the other rows, the split over CTAs or the run.
  * tokens (B2R_I32 or B2R_I64, out_dtype) and logprobs (fp32, may be NULL: log of the probability with which the token
  * was drawn; 0 for T <= 0, -inf for no token) have n_rows elements. Parameters are fp32 / int32 device vectors of
- * n_rows elements, or NULL for the value given for all rows.
+ * n_rows elements, or NULL for the value given for all rows; temperatures above 1e30 count as 1e30. vocab: at most
+ * 16777216.
  */
 typedef struct {
   int32_t dtype;     /* of the logits: B2R_F32, B2R_F16 or B2R_BF16 */

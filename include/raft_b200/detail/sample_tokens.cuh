@@ -45,6 +45,7 @@ constexpr int kMaxPartKb  = 160;  // of a row in a CTA's shared memory
 constexpr int kList       = 2048;
 constexpr int kShort      = 256;  // up to here a list is sorted by comparing all pairs
 constexpr int kScratch    = kList * 12;  // bytes of the row's place in shared memory at least: the sort of a list
+constexpr int kMaxVocab   = 1 << 24;  // the sums of 32 vectors of the largest part (131 KB) fit beside the rest
 constexpr int kMaxShift   = 50;  // weights below 2^51, so that an addition rounds them to integers
 
 template <typename T>
@@ -249,15 +250,6 @@ B2R_DI void cluster_add_u32(unsigned* p, unsigned rank, unsigned v)
 B2R_DI void cluster_max_u32(unsigned* p, unsigned rank, unsigned v)
 {
   asm volatile("red.relaxed.cluster.shared::cluster.max.u32 [%0], %1;" ::"r"(cluster_address(p, rank)), "r"(v) : "memory");
-}
-B2R_DI unsigned cluster_fetch_add_u32(unsigned* p, unsigned rank, unsigned v)
-{
-  unsigned old;
-  asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], %2;"
-               : "=r"(old)
-               : "r"(cluster_address(p, rank)), "r"(v)
-               : "memory");
-  return old;
 }
 B2R_DI void cluster_sync()
 {

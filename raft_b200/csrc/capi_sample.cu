@@ -42,7 +42,7 @@ extern "C" int b2r_sample_tokens(const b2r_sample_desc* desc, void* tokens, floa
   if (desc == nullptr) return B2R_ERR_BAD_ARG;
   const b2r_sample_desc& d = *desc;
   if (d.n_rows < 0 || d.vocab < 0 || d.ld < d.vocab) return B2R_ERR_BAD_ARG;
-  if (d.n_rows > 0x7fffffff || d.vocab > 0x7fffffff - 64) return B2R_ERR_TOO_LARGE;
+  if (d.n_rows > 0x7fffffff || d.vocab > detail::sample::kMaxVocab) return B2R_ERR_TOO_LARGE;
   if (d.n_rows > 0 && (tokens == nullptr || uniform == nullptr || (d.vocab > 0 && logits == nullptr)))
     return B2R_ERR_BAD_ARG;
   if (d.out_dtype != B2R_I32 && d.out_dtype != B2R_I64) return B2R_ERR_UNSUPPORTED;

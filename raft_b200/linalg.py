@@ -593,8 +593,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
 
     logits: [n_rows x vocab] row-major (rows may be strided), float32 / float16 / bfloat16; uniform: float32 [n_rows];
     the parameters are numbers or vectors of n_rows (int32 for top_k, float32 for the others). NaN logits count as
-    -inf; a row of -inf alone gives -1. Returns (tokens, logprobs): int32 or int64, and the float32 log of the
-    probability with which each token was drawn."""
+    -inf; a row of -inf alone gives -1; vocab is at most 16777216. Returns (tokens, logprobs): int32 or int64, and the
+    float32 log of the probability with which each token was drawn."""
     _require_cuda(logits, "logits")
     if logits.dim() != 2:
         raise ValueError("logits must be a matrix")
@@ -618,7 +618,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     k_ptr, k = _sample_param(top_k, "top_k", torch.int32, n, logits)
     p_ptr, p = _sample_param(top_p, "top_p", torch.float32, n, logits)
     m_ptr, m = _sample_param(min_p, "min_p", torch.float32, n, logits)
-    desc = L.SampleDesc(dt, ot, n, vocab, ldl, temp_ptr, k_ptr, p_ptr, m_ptr, temp, min(int(k), 0x7fffffff), p, m)
+    desc = L.SampleDesc(dt, ot, n, vocab, ldl, temp_ptr, k_ptr, p_ptr, m_ptr, temp,
+                        max(0, min(int(k), 0x7fffffff)), p, m)
     with _on(logits.device):
         st = L.load().b2r_sample_tokens(desc, out.data_ptr(), logprobs.data_ptr(), logits.data_ptr(),
                                         uniform.data_ptr(), _stream_ptr(logits.device))

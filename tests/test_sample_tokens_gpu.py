@@ -262,3 +262,21 @@ def test_refusals(cuda):
         linalg.sample_tokens(logits, uniform, out=torch.empty(4, dtype=torch.int16, device=cuda))
     with pytest.raises(_lib.B2RError):
         linalg.sample_tokens(logits.double(), uniform)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_vocabulary(cuda, dtype):
+    logits, uniform, _ = make(3, 1 << 24, dtype, cuda, 5)
+    temperature = torch.tensor([0.0, 0.7, 1.3], device=cuda)
+    check(logits, uniform, temperature, top_k=40)
+    check(logits[1:], uniform[1:].contiguous(), 1.0)
+    with pytest.raises(_lib.B2RError):
+        linalg.sample_tokens(torch.empty((1, (1 << 24) + 1), dtype=dtype, device=cuda), uniform[:1].contiguous())
+
+
+@pytest.mark.parametrize("k", [-1, -2 ** 31, -2 ** 32 + 5, 2 ** 40])
+def test_numbers_of_kept_tokens_beyond_32_bits_keep_all(cuda, k):
+    logits, uniform, _ = make(64, 1000, torch.float32, cuda, 6)
+    got = linalg.sample_tokens(logits, uniform, 1.0, k)
+    exp = linalg.sample_tokens(logits, uniform, 1.0, 0)
+    assert torch.equal(got[0], exp[0]) and torch.equal(got[1], exp[1])

@@ -104,3 +104,9 @@ def test_sample_descriptor_layout_matches_the_header():
     # 2 x int32, 3 x int64, 4 pointers, float, int32, 2 x float = 80 bytes
     assert ctypes.sizeof(L.SampleDesc) == 80
     assert L.SampleDesc.temperature.offset == 32 and L.SampleDesc.temperature_all.offset == 64
+
+
+@pytest.mark.parametrize("vocab,status", [(1 << 24, 1), ((1 << 24) + 1, 4), (0x7fffffff, 4)])
+def test_sample_vocabulary_limit(lib, vocab, status):
+    # (a null `uniform` is refused behind the sizes, so that no call is launched here)
+    assert sample(lib, u=None, vocab=vocab, ld=vocab) == status
