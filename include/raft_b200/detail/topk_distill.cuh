@@ -8,9 +8,8 @@
 // A row without a valid entry (all tokens -1: prompt or padding positions) has loss 0 and gradient 0.
 //
 // The pass over the logits is what costs: V elements per row are read once, and written once where the gradient is
-// wanted. For the gradient a row is spread over the CTAs of a cluster, which keep its exponentials in registers
-// between the two uses, so that no second read is needed; the CTAs exchange (maximum, sum) pairs through distributed
-// shared memory. Sums and statistics are fp32, relative to the maximum; the loss, a sum of k terms, is fp64.
+// wanted. For the gradient a row is spread over the CTAs of a cluster, which keep it in shared memory between the two
+// uses, so that no second read is needed; the CTAs exchange (maximum, sum) pairs through distributed shared memory. Sums and statistics are fp32, relative to the maximum; the loss, a sum of k terms, is fp64.
 #pragma once
 
 #include "launch.cuh"
@@ -391,7 +390,8 @@ B2R_DI bool listed_weight(const int* id, const float* logp, int k, int j, float*
 // to memory. Between the two lies the first pass over the NEXT row, so that nobody waits for the records.
 //
 // Two exponentials per element: 8 elements per clock and SM at the MUFU unit's 16, 4100 clocks of a row's 64 KB part,
-// against 5100 that its 128 KB of traffic take. Keeping the first pass's exponentials instead needs 64 registers of
+// against 5100 that its 128 KB of traffic take. 4096 x 131072 bf16 takes 511 us (4.2 TB/s; clusters of four fit on 132 of
+// the 148 SMs; with the rest of the arithmetic the unit is busy half the time, and the workers never wait). Keeping the first pass's exponentials instead needs 64 registers of
 // every worker for them; ptxas then spills (512 workers of 64 elements: 96 registers, 815 us for 4096 rows of 131072
 // bf16; 256 of 128: 168 registers, 1195 us). Forms before that: workers that copied their own vectors in and out, 750 us
 // (5000 of 12000 clocks per row in the copies); cluster barriers for the exchange, which wait for the gradient's

@@ -129,3 +129,33 @@ def test_a_step_and_the_tokens_behind_it_in_one_graph(cuda, n):
     torch.cuda.synchronize()
     for a, b in zip(again, captured):
         assert torch.equal(a, b)
+
+
+def test_calls_at_once_on_two_streams_from_two_threads(cuda):
+    """Scratch, status words and launch records are shared: each thread's results have to be those it gets alone."""
+    import threading
+    sets = [program(cuda, n, n) for n in (900, 1500)]
+    uniforms = [torch.rand(s[1].numel(), device=cuda) for s in sets]
+
+    def once(s, u):
+        out = step(*s)
+        return [*out, *linalg.sample_tokens(out[1], u, 0.9, 0, 0.95, 0.0)]
+    alone = [once(s, u) for s, u in zip(sets, uniforms)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = once(sets[i], uniforms[i])
+                stream.synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, alone[i])):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    assert linalg.last_kernel_status(cuda) == 0
