@@ -328,3 +328,19 @@ def test_refusals(cuda):
         linalg.embedding_grad(g, tokens, 10, out_dtype=torch.float16)
     with pytest.raises(_lib.B2RError):
         linalg.embedding_grad(g.half(), tokens, 10, out_dtype=torch.bfloat16)
+
+
+def test_refuses_a_broadcast_gradient(cuda):
+    """What a sum's backward pass hands on: every row at the same address."""
+    g = torch.ones(1, 8, device=cuda).expand(4, 8)
+    with pytest.raises(ValueError):
+        linalg.embedding_grad(g, torch.arange(4, device=cuda), 10)
+    assert_grad(linalg.embedding_grad(g.contiguous(), torch.arange(4, device=cuda), 10), g.contiguous(),
+                torch.arange(4, device=cuda), 10, 1.0)
+
+
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 8191, 8192, 8193])
+def test_grad_at_the_borders_between_the_forms(cuda, n):
+    tokens = tokens_of(n, 700, torch.int64, cuda, "skew", n)
+    g = torch.randn((n, 36), generator=torch.Generator(device=cuda).manual_seed(n), device=cuda)
+    assert_grad(linalg.embedding_grad(g, tokens, 700, scale=0.5), g, tokens, 700, 0.5)

@@ -413,3 +413,11 @@ def test_a_record_that_never_arrives_ends_in_nan_and_a_status(cuda, knobs):
     assert linalg.last_kernel_status(cuda) == _lib.OK
     for a, b in zip(again, exp):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k", [799, 800, 801, 1024])
+@pytest.mark.parametrize("vocab", [32768, 131072, 262144])
+def test_long_lists_beside_full_rows(cuda, dtype, k, vocab):
+    """The list takes its place beside the row's buffers in shared memory, or the row is streamed."""
+    run_all(*make(3, vocab, k, dtype, cuda, k), 1.5)
