@@ -314,8 +314,8 @@ B2R_API size_t b2r_embedding_grad_workspace_bytes(int64_t n_tokens, int64_t n_co
  *                         over the logits: one read and one write of the matrix.
  *  b2r_topk_distill_grad  the gradient alone, from the lse of an earlier call.
  * logits and grad have type `dtype`; teacher is B2R_F32, B2R_F16 or B2R_BF16; loss, lse, grad_loss are fp32.
- * k is at most 1024 (B2R_ERR_TOO_LARGE), temperature between 1e-30 and 1e30. `grad` may be `logits` (same pointer and stride), else it must not
- * overlap them. The gradient is written fastest when both matrices start on the same 16-byte phase and have the
+ * k is at most 1024 (B2R_ERR_TOO_LARGE), temperature between 1e-30 and 1e30. `grad` may be `logits` (same pointer
+ * and stride), else it must not overlap them; no output may overlap another input or output. The gradient is written fastest when both matrices start on the same 16-byte phase and have the
  * same stride modulo 16 bytes.
  */
 B2R_API int b2r_topk_distill(float* loss,
@@ -370,8 +370,8 @@ B2R_API int b2r_topk_distill_grad(void* grad,
  * row's token does not depend on the other rows, the split over CTAs or the run.
  * tokens (B2R_I32 or B2R_I64, out_dtype) and logprobs (fp32, may be NULL: log of the probability with which the token
  * was drawn; 0 for T <= 0, -inf for no token) have n_rows elements. Parameters are fp32 / int32 device vectors of
- * n_rows elements, or NULL for the value given for all rows; temperatures above 1e30 count as 1e30. vocab: at most
- * 16777216.
+ * n_rows elements, or NULL for the value given for all rows; temperatures above 1e30 count as 1e30. Outputs must not
+ * overlap inputs. vocab: at most 16777216 (B2R_ERR_TOO_LARGE).
  */
 typedef struct {
   int32_t dtype;     /* of the logits: B2R_F32, B2R_F16 or B2R_BF16 */

@@ -513,8 +513,22 @@ def _grad_like(grad, logits, ldl):
     return grad, ldg
 
 
+def _apart(outputs, inputs):
+    """Refuses given outputs (name, tensor or None) that overlap an input or one another."""
+    for i, (name, out) in enumerate(outputs):
+        if out is None:
+            continue
+        for other_name, other in inputs + outputs[:i]:
+            if other is not None and _overlap(out, other):
+                raise ValueError(f"{name} must not overlap {other_name}")
+
+
 def _distill(where, logits, teacher_ids, teacher_logits, grad_loss, temperature, loss, lse, grad, want_grad):
     dt, it, tt, ldl, ldi, ldt, n, vocab, k = _distill_args(logits, teacher_ids, teacher_logits, temperature, where)
+    if loss is not None or lse is not None or grad is not None:
+        lists = [("teacher_ids", teacher_ids), ("teacher_logits", teacher_logits), ("grad_loss", grad_loss)]
+        _apart([("loss", loss), ("lse", lse)], lists + [("logits", logits)])
+        _apart([("grad", grad)], lists + [("loss", loss), ("lse", lse)])
     loss = torch.empty(n, dtype=torch.float32, device=logits.device) if loss is None else \
         _per_row(loss, "loss", n, logits)
     lse = torch.empty(n, dtype=torch.float32, device=logits.device) if lse is None else _per_row(lse, "lse", n, logits)
@@ -563,6 +577,8 @@ def topk_distill_grad(logits, teacher_ids, teacher_logits, lse, grad_loss, tempe
                                                            "topk_distill_grad")
     _per_row(lse, "lse", n, logits)
     _per_row(grad_loss, "grad_loss", n, logits)
+    _apart([("grad", grad)], [("teacher_ids", teacher_ids), ("teacher_logits", teacher_logits), ("lse", lse),
+                              ("grad_loss", grad_loss)])
     grad, ldg = _grad_like(grad, logits, ldl)
     with _on(logits.device):
         st = L.load().b2r_topk_distill_grad(
@@ -604,6 +620,10 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     n, vocab = logits.shape
     ldl = _row_stride(logits, "logits")
     _per_row(uniform, "uniform", n, logits)
+    if out is not None or logprobs is not None:
+        _apart([("out", out), ("logprobs", logprobs)], [("logits", logits), ("uniform", uniform)] + [
+            (name, v) for name, v in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p),
+                                      ("min_p", min_p)) if isinstance(v, torch.Tensor)])
     if out is None:
         out = torch.empty(n, dtype=index_dtype, device=logits.device)
     _on_device_of(out, "out", logits)

@@ -159,3 +159,26 @@ def test_calls_at_once_on_two_streams_from_two_threads(cuda):
         t.join()
     assert not wrong
     assert linalg.last_kernel_status(cuda) == 0
+
+
+def test_outputs_over_inputs_are_refused(cuda):
+    logits = torch.randn((6, 50), device=cuda)
+    ids = torch.zeros((6, 6), dtype=torch.int64, device=cuda)
+    teacher, weight = torch.zeros((6, 6), device=cuda), torch.ones(6, device=cuda)
+    lse, both = torch.zeros(6, device=cuda), torch.zeros(6, device=cuda)
+    for kw in (dict(loss=weight), dict(lse=weight), dict(loss=both, lse=both), dict(loss=logits[0, :6]),
+               dict(lse=teacher[0]), dict(loss=logits[0, :6], grad=logits)):
+        with pytest.raises(ValueError):
+            linalg.topk_distill_step(logits, ids, teacher, weight, **kw)
+    square = torch.randn((6, 6), device=cuda)
+    with pytest.raises(ValueError):
+        linalg.topk_distill_step(square, ids, teacher, weight, grad=teacher)
+    with pytest.raises(ValueError):
+        linalg.topk_distill_grad(square, ids, teacher, lse, weight, grad=teacher)
+    uniform = torch.rand(6, device=cuda)
+    for kw in (dict(logprobs=uniform), dict(logprobs=logits[0, :6]), dict(temperature=both, logprobs=both),
+               dict(out=both.view(torch.int32), logprobs=both)):
+        with pytest.raises(ValueError):
+            linalg.sample_tokens(logits, uniform, **kw)
+    loss, lse, grad = linalg.topk_distill_step(logits, ids, teacher, weight, loss=both, lse=lse, grad=logits)
+    assert grad is logits and loss is both
