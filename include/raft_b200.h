@@ -315,8 +315,9 @@ B2R_API size_t b2r_embedding_grad_workspace_bytes(int64_t n_tokens, int64_t n_co
  *  b2r_topk_distill_grad  the gradient alone, from the lse of an earlier call.
  * logits and grad have type `dtype`; teacher is B2R_F32, B2R_F16 or B2R_BF16; loss, lse, grad_loss are fp32.
  * k is at most 1024 (B2R_ERR_TOO_LARGE), temperature between 1e-30 and 1e30. `grad` may be `logits` (same pointer
- * and stride), else it must not overlap them; no output may overlap another input or output. The gradient is written fastest when both matrices start on the same 16-byte phase and have the
- * same stride modulo 16 bytes.
+ * and stride), else it must not overlap them; no output may overlap another input or output. The
+ * gradient is written fastest when both matrices start on the same 16-byte phase and have the same stride modulo
+ * 16 bytes.
  */
 B2R_API int b2r_topk_distill(float* loss,
                              float* lse,
