@@ -308,8 +308,9 @@ B2R_API size_t b2r_embedding_grad_workspace_bytes(int64_t n_tokens, int64_t n_co
  *     p = softmax(y / T) over the entries whose token lies in [0, vocab),   q = softmax(z / T) over the vocabulary
  *     loss[r] = T^2 * sum_k p_k (log p_k - log q[ids_k])                    lse[r] = log sum_v exp(z_v / T)
  *     grad[r][v] = grad_loss[r] * T * (q_v - sum of p_k with ids_k == v)    (= grad_loss[r] * d loss[r] / d z_v)
- * A token named twice counts twice. A row without any valid entry, or whose valid entries are all -inf, has loss 0
- * and gradient 0 whatever its logits hold; elsewhere NaN and +inf logits give NaN.
+ * A token named twice counts twice. A p_k that fp32 holds as 0 adds nothing, even where q is 0. A row without any valid
+ * entry, or whose valid entries are all -inf, has loss 0 and gradient 0 whatever its logits hold; elsewhere NaN and +inf
+ * logits give NaN.
  *  b2r_topk_distill       loss and lse (either may be NULL), and with `grad` non-NULL the gradient in the same pass
  *                         over the logits: one read and one write of the matrix.
  *  b2r_topk_distill_grad  the gradient alone, from the lse of an earlier call.

@@ -5,6 +5,7 @@
 //     q = softmax(z / T)       over the vocabulary
 //     loss = T^2 * sum_k p_k (log p_k - log q[id_k]),     lse = log sum_v exp(z_v / T)
 //     d loss / d z_v = T (q_v - sum of p_k with id_k = v)
+// A p_k that fp32 holds as 0 (an entry far below the list's largest) adds nothing, where q is 0 too: not 0 * inf.
 // A row without a valid entry (all tokens -1: prompt or padding positions) has loss 0 and gradient 0.
 //
 // The pass over the logits is what costs: V elements per row are read once, and written once where the gradient is
@@ -590,7 +591,7 @@ distill_step_kernel(const Args<T> a)
         const float zt = FloatIo<T>::up(held[t]);
         const double w = double(expf(lp));
         zid[j]         = zt;
-        sum += lp == -INFINITY ? 0.0 : w * (double(lp) - double(zt) * inverse);
+        sum += w == 0.0 ? 0.0 : w * (double(lp) - double(zt) * inverse);
         share += w;
       }
     });
@@ -933,8 +934,8 @@ distill_stream_kernel(const Args<T> a)
     const double lse = double(all.m) / a.temperature + double(logf(all.s));
     double sum       = 0.0;
     for (int j = lane; j < k && some; j += 32) {
-      if (id[j] >= 0 && !(logp[j] == -INFINITY))
-        sum += double(expf(logp[j])) * (double(logp[j]) - (double(zid[j]) / a.temperature - lse));
+      const double w = double(expf(logp[j]));
+      if (id[j] >= 0 && w != 0.0) sum += w * (double(logp[j]) - (double(zid[j]) / a.temperature - lse));
     }
     sum = warp_sum(sum);
     if (lane == 0) {
