@@ -218,6 +218,13 @@ B2R_DI float max3(float a, float b, float c)
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// NaN if either is
+B2R_DI float max_nan(float a, float b)
+{
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // Two fp32 values handled by one instruction.
 using Pair = unsigned long long;
@@ -992,12 +999,12 @@ distill_grad_kernel(const Args<T> a, unsigned parts)
   const int tid = int(threadIdx.x);
   if (part.n <= 0) return;  // uniform over the CTA
   // 1 / T in two fp32 pieces: rounded to one it would scale the row by its largest logit's share of the error
-  // (-inf is taken as the lowest finite value: -inf times a zero piece would be NaN)
+  // (-inf is taken as the lowest finite value: -inf times a zero piece would be NaN; a NaN stays one)
   const double inv = 1.0 / a.temperature;
   const float hi_t = float(inv), lo_t = float(inv - double(hi_t));
   const float lse = a.lse_in[row];
   const auto q    = [&](float x) {
-    const float f = fmaxf(x, -FLT_MAX);
+    const float f = max_nan(x, -FLT_MAX);
     return ex2(fmaf(f, lo_t, fmaf(f, hi_t, -lse)) * 1.4426950408889634f);
   };
   Words4 raw[NV];
