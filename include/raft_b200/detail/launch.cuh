@@ -159,6 +159,7 @@ struct Tuning {
   int normalize_ctas_per_sm = 0;    // B2R_NORMALIZE_CPS row_normalize CTAs per SM at most (0: 256, short-lived CTAs; 8: two resident waves)
   int wait_limit_ms        = 1000;  // B2R_WAIT_LIMIT_MS bound of every mbarrier wait inside the ring kernels, milliseconds
   int test_skip_tile       = 0;     // B2R_TEST_SKIP_TILE test hook: the producer of the first CTA never requests tile (value - 1)
+  int test_late_warp       = 0;     // B2R_TEST_LATE_WARP test hook of the distillation step: with B2R_TEST_SKIP_TILE, warp (value - 1) of the first CTA takes its wait for that row as run out, and nothing is withheld
 };
 
 inline int env_int(const char* name, int dflt)
@@ -224,6 +225,7 @@ inline Tuning read_tuning_from_env()
   x.normalize_ctas_per_sm = env_int("B2R_NORMALIZE_CPS", x.normalize_ctas_per_sm);
   x.wait_limit_ms        = env_int("B2R_WAIT_LIMIT_MS", x.wait_limit_ms);
   x.test_skip_tile       = env_int("B2R_TEST_SKIP_TILE", x.test_skip_tile);
+  x.test_late_warp       = env_int("B2R_TEST_LATE_WARP", x.test_late_warp);
   return x;
 }
 

@@ -53,6 +53,7 @@ struct Args {
   double temperature;
   int per_cta;  // vectors of a row per CTA of the cluster
   RingCtl ctl;  // bounded waits
+  int late_warp;  // test hook (-1: none): this warp of the first CTA is told that row ctl.skip_tile did not arrive in time
 };
 
 B2R_DI float ex2(float x)
@@ -439,6 +440,7 @@ distill_step_kernel(const Args<T> a)
   __shared__ int some_s[3];
   __shared__ int twice_s[3];  // a token of this CTA's is named twice
   __shared__ int gave_up;
+  __shared__ int missed[kStages];  // somebody did not see the copy into this buffer arrive
   Vec* stages         = reinterpret_cast<Vec*>(step_smem);                   // [kStages][NT * NV]
   const int k         = a.list.k;
   int* ids            = reinterpret_cast<int*>(stages + kStages * NT * NV);  // [3][k]
@@ -452,8 +454,10 @@ distill_step_kernel(const Args<T> a)
   if (tid == 0) {
     for (int i = 0; i < 4; ++i)
       mbar_init(&arrived[i], 1);
-    for (int i = 0; i < kStages; ++i)
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&full[i], 1);
+      missed[i] = 0;
+    }
     gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -479,7 +483,19 @@ distill_step_kernel(const Args<T> a)
   cluster_arrive();  // every CTA of the cluster has started, its barriers are set up
   grid_dep_sync();
 
-  // ---- sender
+  const int late_row = blockIdx.x == 0 && warp == a.late_warp ? a.ctl.skip_tile : -1;
+  bool there = true;  // everything that this warp has waited for so far has arrived
+  // Whether row number n of this cluster, on its way into buffer `stage`, has arrived. The copy may still land after a
+  // wait that ran out, over whatever the buffer holds then: `missed` keeps the buffer from becoming a gradient.
+  auto landed = [&](int n, int stage, unsigned phase) {
+    const bool late = n == late_row;
+    if (late) *static_cast<volatile int*>(&gave_up) = 1;
+    const bool here = there && !late && mbar_wait_bounded(&full[stage], phase, &gave_up, a.ctl.limit_ns);
+    if (!here) *static_cast<volatile int*>(&missed[stage]) = 1;
+    return here;
+  };
+
+  // ---- mover
   // row's vectors on their way into buffer `stage` (all lanes of the warp come here)
   auto request = [&](int64_t row, int stage) {
     if (row >= a.n_rows) return;
@@ -505,6 +521,17 @@ distill_step_kernel(const Args<T> a)
     if (lane == 0 && part.hi > part.lo && same_phase(g, a.logits + row * a.ldl))
       bulk_store(g + part.first + part.lo * VE, stages + stage * (NT * NV) + part.lo, unsigned(part.hi - part.lo) * 16u);
   };
+  // NaN over what has become of a row that somebody missed
+  auto take_back = [&](int64_t row) {
+    bulk_store_wait_all();
+    __syncwarp();
+    const RowPart<T> part = part_of(row);
+    T* g                  = a.grad + row * a.ldg;
+    for (int64_t t = part.token0 + lane; t < part.token1; t += 32)
+      g[t] = FloatIo<T>::down(NAN);
+  };
+
+  // ---- sender
   // the record of a row whose parts the workers have left in warp_part (all lanes); n: the row's number here
   auto send = [&](int n, int buf) {
     const float2 v = lane < NW ? warp_part[lane] : make_float2(-INFINITY, 0.0f);
@@ -512,7 +539,8 @@ distill_step_kernel(const Args<T> a)
     const long long bits = __double_as_longlong(list_sums[buf][0]);
     const float4 rec = make_float4(w.m, w.s, __int_as_float(int(bits)), __int_as_float(int(bits >> 32)));
     const int at     = n & 3;
-    const bool skip  = blockIdx.x == 0 && n == a.ctl.skip_tile;  // test hook: this record is never sent
+    // test hook: this record is never sent
+    const bool skip = blockIdx.x == 0 && n == a.ctl.skip_tile && a.late_warp < 0;
     if (size == 1) {
       if (lane == 0 && !skip) {
         record[at][0]   = rec;
@@ -542,7 +570,7 @@ distill_step_kernel(const Args<T> a)
       if (u * 32 + lane < k) ahead[u].ask(a, row, u * 32 + lane);
     ahead_weight = a.grad_loss[row];
   };
-  auto prepare = [&](int64_t row, int buf, int stage, unsigned phase) {
+  auto prepare = [&](int64_t row, int n, int buf, int stage, unsigned phase) {
     if (row >= a.n_rows) return;
     const RowPart<T> part = part_of(row);
     int* id               = ids + buf * k;
@@ -585,7 +613,7 @@ distill_step_kernel(const Args<T> a)
     each([&](int, int, float& y) { total += some ? expf((y - m) * inv_t) : 0.0f; });
     const float ls = logf(warp_sum(total));
     // the row itself, for the student's logits of the listed tokens
-    const bool here = mbar_wait_bounded(&full[stage], phase, &gave_up, a.ctl.limit_ns);
+    const bool here = landed(n, stage, phase);
     const T* held   = reinterpret_cast<const T*>(stages + stage * (NT * NV)) - part.first;  // held[t]: token t
     double sum = 0.0, share = 0.0;
     bool twice = false;
@@ -624,15 +652,15 @@ distill_step_kernel(const Args<T> a)
   };
 
   // ---- workers
-  bool there = true;  // everything waited for so far has arrived
-  // (m, s) of the warp's elements of the row in buffer `stage`
-  auto first_pass = [&](int n, int stage, unsigned phase) {
-    there = there && mbar_wait_bounded(&full[stage], phase, &gave_up, a.ctl.limit_ns);
+  // (m, s) of the warp's elements of row number n here, which lies in buffer `stage`
+  auto first_pass = [&](int64_t row, int n, int stage, unsigned phase) {
+    const int n_vec = part_of(row).n;
+    there           = landed(n, stage, phase);
     const Vec* mine = stages + stage * (NT * NV) + tid;
     float m = -INFINITY, s = 0.0f;
 #pragma unroll
     for (int i0 = 0; i0 < NV; i0 += CV) {
-      if (i0 * NT + warp * 32 >= n) break;
+      if (i0 * NT + warp * 32 >= n_vec) break;
       Pair e[CP];
       float top = m;
 #pragma unroll
@@ -660,7 +688,7 @@ distill_step_kernel(const Args<T> a)
       const float2 s2 = split(add2(sum0, sum1));
       s               = s2.x + s2.y;
     }
-    const ExpSum w = warp_join({m, s}, c);
+    const ExpSum w = warp_join({m, there ? s : NAN}, c);
     if (lane == 0) warp_part[warp] = make_float2(w.m, w.s);
   };
   // the gradient of the row in buffer `stage`, written over it (vectors that are not whole, or whose row in memory has
@@ -747,9 +775,9 @@ distill_step_kernel(const Args<T> a)
   }
   __syncthreads();
   if (warp == NW + 1) ask(first);
-  if (warp == NW + 1) prepare(first, 0, 0, 0);
-  if (warp == NW + 1) prepare(first + step, 1, 1, 0);
-  if (warp < NW) first_pass(part_of(first).n, 0, 0);
+  if (warp == NW + 1) prepare(first, 0, 0, 0, 0);
+  if (warp == NW + 1) prepare(first + step, 1, 1, 1, 0);
+  if (warp < NW) first_pass(first, 0, 0, 0);
   cluster_wait();
   __syncthreads();
   if (warp == NW) send(0, 0);
@@ -764,7 +792,7 @@ distill_step_kernel(const Args<T> a)
     const unsigned phase  = unsigned(n >> 2) & 1u;  // of the records
     bool listed = false;
     if (warp < NW) {
-      if (row + step < a.n_rows) first_pass(part_of(row + step).n, nxt, nround);
+      if (row + step < a.n_rows) first_pass(row + step, n + 1, nxt, nround);
       handover();
       second_pass(row, n, cur, cur, phase);
     } else if (warp == NW) {
@@ -773,7 +801,7 @@ distill_step_kernel(const Args<T> a)
       listed = some_s[cur] != 0;
     } else if (warp == NW + 1 && there) {
       // (the list of the row after the next goes where the row before had its)
-      prepare(row + 2 * step, nn, nn, nn == 0 || nxt == 0 ? round ^ 1u : round);
+      prepare(row + 2 * step, n + 2, nn, nn, nn == 0 || nxt == 0 ? round ^ 1u : round);
     }
     __syncthreads();
     if (warp == NW + 2) {
@@ -781,7 +809,10 @@ distill_step_kernel(const Args<T> a)
       bulk_store_wait_read();  // (by the lane that stores)
       __syncwarp();
       // (after a give-up nothing says that the buffer's last copy has landed)
-      if (*static_cast<volatile int*>(&gave_up) == 0) request(row + 3 * step, cur);
+      if (!__any_sync(kFull, *static_cast<volatile int*>(&gave_up) != 0))  // (the warp as a whole, whenever it is set)
+        request(row + 3 * step, cur);
+      else if (missed[cur] != 0)
+        take_back(row);
     } else if (warp == NW) {
       there = there && mbar_wait_bounded(&arrived[n & 3], phase, &gave_up, a.ctl.limit_ns);
       if (rank == 0) {
@@ -809,7 +840,8 @@ distill_step_kernel(const Args<T> a)
         (void)mbar_drain_bounded(&full[i], i < cur ? round : round ^ 1u, a.ctl.limit_ns);
     }
   }
-  if (!there && tid == 0) ring_report_timeout(a.ctl);
+  __syncthreads();
+  if (tid == 0 && gave_up != 0) ring_report_timeout(a.ctl);  // whoever it was
   if (size > 1) {  // nobody sends to a CTA that has left
     cluster_arrive();
     cluster_wait();

@@ -40,6 +40,7 @@ static detail::distill::Args<T> distill_args(const void* logits, int64_t ldl, vo
   a.vocab       = int(vocab);
   a.temperature = temperature;
   a.ctl         = detail::ring_ctl(kernel_status_word());
+  a.late_warp   = detail::tuning().test_late_warp - 1;
   return a;
 }
 
