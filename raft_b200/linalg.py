@@ -345,14 +345,27 @@ def _row_stride(t, name):
 
 
 def _overlap(a, b):
-    """Whether the memory that two tensors span overlaps."""
-    def span(t):
-        if t.numel() == 0:
-            return 0, 0
-        lo = t.data_ptr()
-        return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    """Whether two tensors share memory. Rows of a matrix may lie between rows of another (column blocks of one buffer);
+    of layouts that are not matrices of contiguous rows apart from one another, the memory that they span counts."""
+    def rows(t):  # (address of the first row, bytes of a row, distance of rows, number of rows)
+        size = t.element_size()
+        if t.dim() == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) > t.shape[1]:
+            return t.data_ptr(), t.shape[1] * size, t.stride(0) * size, t.shape[0]
+        return t.data_ptr(), (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * size, 0, 1
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, la, sa, na), (b0, lb, sb, nb) = rows(a), rows(b)
+    if a0 >= b0 + (nb - 1) * sb + lb or b0 >= a0 + (na - 1) * sa + la:
+        return False
+    if na < nb:
+        (a0, la, sa, na), (b0, lb, sb, nb) = (b0, lb, sb, nb), (a0, la, sa, na)
+    if na == 1:
+        return True
+    # for every row of b: is there an i such that row a0 + i sa begins before its end and ends behind its beginning?
+    begin = b0 - a0 + torch.arange(nb, dtype=torch.int64) * sb
+    first = torch.div(begin - la, sa, rounding_mode="floor") + 1
+    last = torch.div(begin + lb - 1, sa, rounding_mode="floor")
+    return bool((first.clamp(min=0) <= last.clamp(max=na - 1)).any())
 
 
 def _workspace(workspace, like):
