@@ -512,11 +512,14 @@ def _per_row(t, name, n, logits):
 
 
 def _grad_like(grad, logits, ldl):
-    """`grad`, checked, or a new matrix with logits' row stride (so that rows of both have the same alignment)."""
+    """`grad`, checked, or a new matrix whose row stride differs from logits' by a multiple of 16 bytes (so that rows of
+    both have the same alignment) and is as short as that allows: logits may be rows far apart, the last positions of
+    sequences, say."""
     if grad is None:
         n, vocab = logits.shape
-        grad = torch.empty_strided((n, vocab), (max(ldl, 1), 1), dtype=logits.dtype, device=logits.device)
-        return grad, ldl
+        ldg = vocab + (ldl - vocab) % (16 // logits.element_size())
+        grad = torch.empty_strided((n, vocab), (max(ldg, 1), 1), dtype=logits.dtype, device=logits.device)
+        return grad, ldg
     _on_device_of(grad, "grad", logits)
     if grad.dtype != logits.dtype or grad.shape != logits.shape:
         raise ValueError("grad must have the shape and element type of logits")
