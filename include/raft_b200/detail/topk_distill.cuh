@@ -639,9 +639,11 @@ distill_step_kernel(const Args<T> a)
       share += __shfl_xor_sync(kFull, share, o);
     }
     twice = __any_sync(kFull, twice);
+    __syncwarp();  // the bits are cleared when all lanes have asked for theirs, and asked for again when they are clear
     each([&](int, int t, float&) {
       if (t >= part.token0 && t < part.token1) seen[unsigned(t - part.first) >> 5] = 0;
     });
+    __syncwarp();
     if (lane == 0) {
       twice_s[buf]      = twice;
       list_sums[buf][0] = here ? sum : double(NAN);
