@@ -310,10 +310,12 @@ B2R_API size_t b2r_embedding_grad_workspace_bytes(int64_t n_tokens, int64_t n_co
  *     grad[r][v] = grad_loss[r] * T * (q_v - sum of p_k with ids_k == v)    (= grad_loss[r] * d loss[r] / d z_v)
  * A token named twice counts twice. A p_k that fp32 holds as 0 adds nothing, even where q is 0. A row without any valid
  * entry, or whose valid entries are all -inf, has loss 0 and gradient 0 whatever its logits hold; elsewhere NaN and +inf
- * logits give NaN.
+ * logits, and rows of -inf alone, give NaN.
  *  b2r_topk_distill       loss and lse (either may be NULL), and with `grad` non-NULL the gradient in the same pass
  *                         over the logits: one read and one write of the matrix.
- *  b2r_topk_distill_grad  the gradient alone, from the lse of an earlier call.
+ *  b2r_topk_distill_grad  the gradient alone, from the lse of an earlier call. Its q carry the rounding of the fp32 lse, a
+ *                         factor of 1 +- |lse| 2^-24 (4 10^-4 for logits of 70 at T = 0.01; at most 1 in all), which
+ *                         the gradient of b2r_topk_distill does not: take that one at low temperatures.
  * logits and grad have type `dtype`; teacher is B2R_F32, B2R_F16 or B2R_BF16; loss, lse, grad_loss are fp32.
  * k is at most 1024 (B2R_ERR_TOO_LARGE), temperature between 1e-30 and 1e30. `grad` may be `logits` (same pointer
  * and stride), else it must not overlap them; no output may overlap another input or output. The

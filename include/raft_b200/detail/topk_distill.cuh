@@ -226,6 +226,12 @@ B2R_DI float max_nan(float a, float b)
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+B2R_DI float min_nan(float a, float b)
+{
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 // Two fp32 values handled by one instruction.
 using Pair = unsigned long long;
@@ -1036,10 +1042,13 @@ distill_grad_kernel(const Args<T> a, unsigned parts)
   // (-inf is taken as the lowest finite value: -inf times a zero piece would be NaN; a NaN stays one)
   const double inv = 1.0 / a.temperature;
   const float hi_t = float(inv), lo_t = float(inv - double(hi_t));
-  const float lse = a.lse_in[row];
-  const auto q    = [&](float x) {
+  // (a row of -inf alone has no probabilities)
+  const float lse = a.lse_in[row] == -INFINITY ? NAN : a.lse_in[row];
+  // The fp32 lse is off by up to |lse| 2^-24, which at low temperatures is more than 1: a probability never is.
+  const auto q = [&](float x) {
     const float f = max_nan(x, -FLT_MAX);
-    return ex2(fmaf(f, lo_t, fmaf(f, hi_t, -lse)) * 1.4426950408889634f);
+    const float d = min_nan(fmaf(f, lo_t, fmaf(f, hi_t, -lse)), 0.0f);
+    return ex2(fmaf(f, 0.0f, d * 1.4426950408889634f));  // (NaN for +inf)
   };
   Words4 raw[NV];
   if (tid < NT) {

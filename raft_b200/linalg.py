@@ -588,7 +588,8 @@ def topk_distill_step(logits, teacher_ids, teacher_logits, grad_loss, temperatur
 def topk_distill_grad(logits, teacher_ids, teacher_logits, lse, grad_loss, temperature=1.0, grad=None):
     """The gradient of topk_distill alone, from the lse that it returned:
     grad[r, v] = grad_loss[r] * T * (softmax(logits / T)[r, v] - sum of p_k with teacher_ids[r, k] == v).
-    `grad` may be `logits`. Returns grad."""
+    The softmax carries the rounding of the float32 lse, a factor of 1 +- |lse| 2^-24; where that is too much (low
+    temperatures, large logits) topk_distill_step has the gradient without it. `grad` may be `logits`. Returns grad."""
     dt, it, tt, ldl, ldi, ldt, n, vocab, k = _distill_args(logits, teacher_ids, teacher_logits, temperature,
                                                            "topk_distill_grad")
     _per_row(lse, "lse", n, logits)
