@@ -397,7 +397,6 @@ struct SumShape {
   int64_t runs;
   unsigned sum_ctas;   // CTAs that sum, all slabs together
   int64_t zero_rows;   // table rows of a zeroing CTA (0: accumulating, no zeroing)
-  unsigned zero_ctas;
 };
 
 // Sorted rows [run * shape.run, ...) in one group of threads; columns V per thread.
@@ -754,8 +753,7 @@ inline cudaError_t launch_sum(OutT* out, int64_t ldo, float* partial, const InT*
     zero_ctas = ceil_div<int64_t>(vocab, s.zero_rows);
   }
   if (sum_ctas + zero_ctas > int64_t(0x7fffffff) || slabs > int64_t(0x7fffffff)) return cudaErrorInvalidValue;
-  s.sum_ctas  = unsigned(sum_ctas);
-  s.zero_ctas = unsigned(zero_ctas);
+  s.sum_ctas = unsigned(sum_ctas);
   if (sum_ctas + zero_ctas == 0) return cudaSuccess;
   (void)launch_dep(sum_rows_kernel<InT, OutT, V, U>, dim3(unsigned(sum_ctas + zero_ctas)), dim3(kSumThreads), 0, stream,
                    out, ldo, partial, g, ldg, skey, spos, n, n_cols, unsigned(vocab), scale, accumulate, s);

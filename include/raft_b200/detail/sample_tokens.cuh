@@ -508,15 +508,14 @@ sample_kernel(const Args<T> a)
   };
   // The border of the order at which the sum of value(key) over the kept tokens reaches `target` (at least 1, at most
   // the whole sum): its key in *border, the sum over larger keys in *above. With kCount the values are 1.
-  // A target above the whole sum, which is returned in *total: the border is below every kept key, false. With fewer
-  // `digits` than keys have, the border's first ones.
-  auto select = [&](auto count, auto value, auto target_of, int digits, unsigned* border, u64* above, u64* total) {
+  // A target above the whole sum, which is returned in *total: the border is below every kept key, false.
+  auto select = [&](auto count, auto value, auto target_of, unsigned* border, u64* above, u64* total) {
     constexpr bool kCount = decltype(count)::value;
     unsigned prefix = 0;  // bits of the border found so far
     int left        = K::kBits;
     u64 over        = 0;
     u64 target      = 0;
-    while (left > 0 && digits-- > 0) {
+    while (left > 0) {
       const int bits  = left > kDigitBits ? kDigitBits : left;
       const int shift = left - bits;
       const int n     = 1 << bits;
@@ -920,7 +919,7 @@ sample_kernel(const Args<T> a)
   if (by_k) {
     unsigned border;
     u64 above, total;
-    if (select(std::true_type{}, weight, [&](u64) { return u64(top_k); }, 4, &border, &above, &total)) {
+    if (select(std::true_type{}, weight, [&](u64) { return u64(top_k); }, &border, &above, &total)) {
       tau = border;
       limit_ties(u64(top_k) - above);
     }
@@ -938,7 +937,7 @@ sample_kernel(const Args<T> a)
       if (target > whole) target = whole;
       return target;
     };
-    if (select(std::false_type{}, weight, target_of, 4, &border, &above, &total)) {
+    if (select(std::false_type{}, weight, target_of, &border, &above, &total)) {
       const bool same = border == tau;
       const u64 w     = weight(border);
       tau             = border;
