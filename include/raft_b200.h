@@ -258,8 +258,8 @@ B2R_API int b2r_matrix_argmax(void* out,
  * Sizes are at most 2^31 - 1 (B2R_ERR_TOO_LARGE above), offsets are 64-bit.
  *
  * b2r_embedding_lookup:  out[i][0..n_cols) = scale * table[tokens[i]][0..n_cols). A token outside [0, vocab) is no
- * token (padding): its row of `out` is zero and nothing is read for it. out and table have the same type and must
- * not overlap.
+ * token (padding): its row of `out` is zero, whatever the table holds (the table's first row may be read for it). out
+ * and table have the same type and must not overlap.
  */
 B2R_API int b2r_embedding_lookup(void* out,
                                  int64_t ldo,

@@ -3,8 +3,8 @@
 //   lookup   out[i, :] = scale * table[token_i, :]                      (a row of zeros where the token is none)
 //   gradient G[v, :] (+)= scale * sum over i with token_i = v of g[i, :]
 //
-// A token outside [0, vocab) - the usual -1 of padded positions - is no token: nothing is read for it and it
-// adds to nothing.
+// A token outside [0, vocab) - the usual -1 of padded positions - is no token: its row of the lookup is zero whatever the
+// table holds, and it adds to nothing.
 //
 // The gradient is a keyed row sum with as many keys as the vocabulary has tokens, so the scheme of the keyed row
 // sums (an accumulator row per key and work unit) does not carry over: here almost every key has no row at all or
@@ -229,7 +229,8 @@ radix_scatter_kernel(unsigned* okey, unsigned* opos, const TokT* tokens, const u
   const int64_t part = (ceil_div<int64_t>(tile, kRadixWarps) + 31) / 32 * 32;
   int64_t wlo        = lo + int64_t(warp) * part;
   int64_t whi        = wlo + part < hi ? wlo + part : hi;
-  // the warp's first kRadixHeld x 32 rows are kept in registers between counting and placing (all of them, in tiles of up to 2048)
+  // the warp's first kRadixHeld x 32 rows are kept in registers between counting and placing (all of them, in tiles of
+  // up to 2048)
   unsigned held_k[kRadixHeld], held_p[kRadixHeld];
 #pragma unroll
   for (int u = 0; u < kRadixHeld; ++u) {
@@ -575,7 +576,10 @@ fold_rows_kernel(OutT* out, int64_t ldo, const float* partial, const unsigned* s
 // ---------------------------------------------------------------------------------------
 // Short inputs: one launch. A CTA looks after a range of the table's rows: it picks the positions that name them out of
 // all tokens (read once), sorts them (by row, then by position), and its groups of threads take the rows that are named
-// in turn, adding up in the order of the positions; the other rows are zeroed. No scratch.
+// in turn, adding up in the order of the positions; the other rows are zeroed. No scratch. 512 tokens into 32000 x 1024
+// bf16: 20.4 us, of which zeroing takes 10 at the memory's rate; every CTA picks and sorts before it writes its first
+// zero. One group takes all the positions of a row: 1024 equal tokens of 4096 columns take 486 us, 1025, which are
+// sorted and summed in runs, 24.
 // ---------------------------------------------------------------------------------------
 constexpr int kSmallThreads = 512;
 constexpr int kSmallMax     = 1024;

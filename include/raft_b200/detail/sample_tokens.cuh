@@ -8,7 +8,8 @@
 //
 // Which side of a border a token falls on is decided by sums over the vocabulary in which a token may weigh 1e-6 of
 // the whole, so weights are computed in fp64 and summed as INTEGERS of 2^-shift, shift = 62 - ceil(log2 vocab) but at
-// most kMaxShift (45 bits for 131072 tokens): exact, the same whatever the order, the split of the row or the number of rows of the call.
+// most kMaxShift (45 bits for 131072 tokens): exact, the same whatever the order, the split of the row or the number of
+// rows of the call.
 //
 // A cluster of CTAs takes a row, every CTA a part, which it keeps in shared memory. What is kept is nearly always a short
 // beginning of the order, and the work is in not touching the rest more than once or twice, two elements at a time:
@@ -21,7 +22,11 @@
 //   - the elements above the bound, if they are at most kList, are collected in the first CTA, sorted, and the rest
 //     happens there; the other CTAs are done.
 // Longer beginnings (a flat distribution, a large k) are narrowed by radix selection over all elements, a digit at a
-// time, by counts or weights summed over the cluster through distributed shared memory, and drawn from in place.
+// time, by counts or weights summed over the cluster through distributed shared memory, and drawn from in place: 256 rows
+// of 131072 bf16 with a top-k of 50 take 54 us, with a top-p of 0.9 over a body of thousands of tokens 452 (fp32: 98, 608).
+// The bins are of keys, not of values, and end 16 octaves below the largest logit, at zero at the latest: where a row's
+// largest logit is 0 (its maximum subtracted) or little above, few maxima lie in them, no bound is found, and the row
+// takes the long way, or the slow sort below: results are the same, the top-k of 50 takes 199 us (fp32: 340).
 #pragma once
 
 #include "launch.cuh"
@@ -394,8 +399,10 @@ sample_kernel(const Args<T> a)
     return;
   }
   // 2^x by table and polynomial: x * 32 = n + r, 2^x = 2^(n / 32) 2^(r / 32), the second by its Taylor series to the
-  // fifth power (|r / 32| <= 1 / 64: 3e-15), the first from `powers` and an exponent (P. T. P. Tang, 1989). What rounds
-  // to 0 is cut off at `low` (and NaN there is none); temperatures above 1e30 count as that.
+  // fifth power, the first from `powers` and an exponent (P. T. P. Tang, 1989). With |r / 32 ln 2| <= ln 2 / 64 the
+  // series is off by 2.3e-15 of its value, the roundings by four of 2^-53 and, for the exponent's (difference, slope and
+  // product), |ln w| 2^-51: no weight by more than 2^-48 of the largest, before it is rounded to an integer. What
+  // rounds to 0 is cut off at `low` (and NaN there is none); temperatures above 1e30 count as that.
   const double zmax    = double(K::value(kmax));
   const double slope   = 1.4426950408889634 / double(fminf(temp, 1e30f));
   const double slope32 = slope * 32.0;
@@ -621,7 +628,6 @@ sample_kernel(const Args<T> a)
       if (all[r] != 0) last = int(all[r]) - 1;
   };
 
-  // The lowest bin of the first digit that can hold kept tokens, and the number of tokens from it up.
   // w >= min_p, as a bound on the key
   const double mp     = min_p < 1.0f ? double(min_p) : 1.0;
   const unsigned kmin = !by_min ? 0u : (mp == 1.0 ? kmax : min(kmax, K::at_least(zmax + log2(mp) / slope)));
@@ -712,7 +718,8 @@ sample_kernel(const Args<T> a)
         return;
       }
       // into bins, by counts; then every token looks for its place among those of its bin, nearly always a few (a
-      // sorting network over 2048 places takes 14 us, mostly shuffles; this 2)
+      // sorting network over 2048 places takes 14 us, mostly shuffles; this 2). Where no bound was found the bins span
+      // the type's whole range and one holds all, so that all pairs are compared: 256 x 2000 fp32, top-k 1000, 223 us.
       u64* spread     = reinterpret_cast<u64*>(sample_smem);              // [kList]
       unsigned* start = reinterpret_cast<unsigned*>(spread + kList);      // [kList]
 #pragma unroll

@@ -10,7 +10,8 @@
 //
 // The pass over the logits is what costs: V elements per row are read once, and written once where the gradient is
 // wanted. For the gradient a row is spread over the CTAs of a cluster, which keep it in shared memory between the two
-// uses, so that no second read is needed; the CTAs exchange (maximum, sum) pairs through distributed shared memory. Sums and statistics are fp32, relative to the maximum; the loss, a sum of k terms, is fp64.
+// uses, so that no second read is needed; the CTAs exchange (maximum, sum) pairs through distributed shared memory.
+// Sums and statistics are fp32, relative to the maximum; the loss, a sum of k terms, is fp64.
 #pragma once
 
 #include "launch.cuh"
@@ -405,12 +406,12 @@ B2R_DI bool listed_weight(const int* id, const float* logp, int k, int j, float*
 // to memory. Between the two lies the first pass over the NEXT row, so that nobody waits for the records.
 //
 // Two exponentials per element: 8 elements per clock and SM at the MUFU unit's 16, 4100 clocks of a row's 64 KB part,
-// against 5100 that its 128 KB of traffic take. 4096 x 131072 bf16 takes 511 us (4.2 TB/s; clusters of four fit on 132 of
-// the 148 SMs; with the rest of the arithmetic the unit is busy half the time, and the workers never wait). Keeping the first pass's exponentials instead needs 64 registers of
-// every worker for them; ptxas then spills (512 workers of 64 elements: 96 registers, 815 us for 4096 rows of 131072
-// bf16; 256 of 128: 168 registers, 1195 us). Forms before that: workers that copied their own vectors in and out, 750 us
-// (5000 of 12000 clocks per row in the copies); cluster barriers for the exchange, which wait for the gradient's
-// stores, 1350 us.
+// against 5100 that its 128 KB of traffic take. 4096 x 131072 bf16 takes 513 us (4.2 TB/s; clusters of four fit on 132
+// of the 148 SMs, with 19 warps each; neither the exponential unit, 51 %, nor the memory, 41 %, is the limit). Keeping
+// the first pass's exponentials instead needs 64 registers of every worker for them; ptxas then spills (512 workers of 64
+// elements: 96 registers, 815 us for 4096 rows of 131072 bf16; 256 of 128: 168 registers, 1195 us). Forms before that:
+// workers that copied their own vectors in and out, 750 us (5000 of 12000 clocks per row in the copies); cluster barriers
+// for the exchange, which wait for the gradient's stores, 1350 us.
 //
 // Three warps work beside the workers, so that no chain of loads is on the workers' path:
 //   the sender   joins the CTA's (m, s), sends the record, and in the first CTA writes the loss;
@@ -418,6 +419,10 @@ B2R_DI bool listed_weight(const int* id, const float* logp, int k, int j, float*
 //   the lister   prepares the list of the row after the next: weights, the student's logits of the listed tokens, and
 //                the sums A = sum p (log p - z / T), P = sum p over the tokens this CTA holds, of which the loss is
 //                T^2 (A + P lse). (The listed elements of the gradient are written by the warp that holds them.)
+//
+// Every wait is bounded. Whoever gives up sets `gave_up`, by which the CTA reports at its end. A warp that did not see
+// its row come in leaves NaN in the row's record and marks the buffer as missed; the mover then writes NaN over the
+// CTA's part of that row and asks for no further ones.
 //
 // kEven: all rows have the phase of the first, so that the geometry is worked out once.
 // ---------------------------------------------------------------------------------------
@@ -857,10 +862,10 @@ distill_step_kernel(const Args<T> a)
 }
 
 // ---------------------------------------------------------------------------------------
-// Rows that do not fit the registers of a cluster (kGrad), and the loss alone: NT threads stream their CTA's part of
-// the row through shared memory (every thread its own vectors, kStreamDepth - 1 chunks of kStreamNv vectors under way),
+// Gradients whose rows or lists do not fit the shared memory of a cluster (kGrad), and the loss alone: NT threads stream
+// their CTA's part of the row through shared memory (every thread its own vectors, kStreamDepth - 1 chunks of kStreamNv vectors under way),
 // and one more warp of rank 0's CTA takes the list. With kGrad every part is read a second time. Chunks are short so that
-// four CTAs fit an SM and one's beginning lies behind the others' chunks: 2048 x 131072 bf16 takes 115 us (4.7 TB/s),
+// four CTAs fit an SM and one's beginning lies behind the others' chunks: 2048 x 131072 bf16 takes 113 us (4.8 TB/s),
 // 141 with chunks of eight vectors and two CTAs per SM, 130 with four vectors and a fourth stage.
 // ---------------------------------------------------------------------------------------
 constexpr int kStreamNv    = 4;
@@ -1223,7 +1228,9 @@ inline cudaError_t launch_stream(Args<T> a, int64_t most, int size, cudaStream_t
 }
 
 // Loss and gradient: a row is held by the CTAs of a cluster, 4096 vectors (64 KB) each; small vocabularies take small
-// CTAs, and a row of more than 8 full ones is read twice, as are rows whose list does not fit beside the buffers.
+// CTAs, and a row of more than 8 full ones is read twice, as are rows whose list does not fit beside the buffers
+// (1024 x 262144 fp32: 488 us, 2.2 TB/s of one read and one write; 2048 x 32000 bf16 with 1000 entries: 2360 us, as every
+// CTA compares its listed tokens with the whole list).
 template <typename T>
 inline cudaError_t launch_loss_and_grad(const Args<T>& a, cudaStream_t stream)
 {
@@ -1238,7 +1245,8 @@ inline cudaError_t launch_loss_and_grad(const Args<T>& a, cudaStream_t stream)
 
 // Loss: rows are split over up to 8 CTAs, of at least four chunks each, while there are fewer than eight CTAs per SM
 // (2048 x 131072 bf16: 115 us; split in two, with sixteen CTAs per SM, 120, and in four 138: what a CTA does before its
-// first chunk and after its last one is not hidden by the others).
+// first chunk and after its last one is not hidden by the others. The rule was swept there alone; by it 512 x 131072 fp32
+// takes 52 us and 16384 x 32000 bf16 239, 1.25 and 1.47 times what their bytes take).
 template <typename T>
 inline cudaError_t launch_loss(const Args<T>& a, cudaStream_t stream)
 {

@@ -15,6 +15,9 @@ the reference:
 Beside them, without a counterpart in the reference, the vocabulary operators: embedding_lookup, embedding_grad,
 topk_distill, topk_distill_grad, topk_distill_step and sample_tokens.
 
+No function here takes part in autograd: results have no graph, also where an input requires a gradient.
+embedding_grad and topk_distill_grad are the backward passes of embedding_lookup and topk_distill.
+
 Shape errors raise ValueError where the reference's RAFT_EXPECTS raises raft::logic_error;
 unsupported type / operator combinations raise B2RError (raft::exception in the reference).
 Functors are named by strings because a C ABI cannot carry a device lambda; the C++ headers
@@ -383,7 +386,7 @@ def embedding_lookup(table, tokens, scale=1.0, out=None):
     table: [vocab x n_cols] row-major (rows may be strided), float32 / float16 / bfloat16; tokens: int32 / int64 of
     any shape, contiguous; out: [tokens.numel() x n_cols] of the table's type (default: a new tensor of shape
     tokens.shape + (n_cols,)). A token outside [0, vocab) - the -1 of padded positions - gives a row of zeros.
-    Returns out."""
+    Outside autograd (embedding_grad is the gradient). Returns out."""
     _require_cuda(table, "table")
     if table.dim() != 2:
         raise ValueError("table must be a matrix")
@@ -570,7 +573,8 @@ def topk_distill(logits, teacher_ids, teacher_logits, temperature=1.0, loss=None
 
     logits: [n_rows x vocab] row-major (rows may be strided), float32 / float16 / bfloat16; teacher_ids: [n_rows x k]
     int32 / int64, -1 where a list is shorter than k; teacher_logits: [n_rows x k], any of the three types; k <= 1024.
-    A row without a valid entry has loss 0. Returns (loss, lse), float32 vectors."""
+    A row without a valid entry has loss 0. Outside autograd (topk_distill_grad is the gradient, topk_distill_step
+    returns both). Returns (loss, lse), float32 vectors."""
     loss, lse, _ = _distill("topk_distill", logits, teacher_ids, teacher_logits, None, temperature, loss, lse, None,
                             False)
     return loss, lse
