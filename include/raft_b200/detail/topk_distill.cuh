@@ -822,9 +822,10 @@ distill_step_kernel(const Args<T> a)
       bulk_store_wait_read();  // (by the lane that stores)
       __syncwarp();
       // (after a give-up nothing says that the buffer's last copy has landed)
-      if (!__any_sync(kFull, *static_cast<volatile int*>(&gave_up) != 0))  // (the warp as a whole, whenever it is set)
+      // (both flags may be set meanwhile: the warp decides as a whole)
+      if (!__any_sync(kFull, *static_cast<volatile int*>(&gave_up) != 0))
         request(row + 3 * step, cur);
-      else if (missed[cur] != 0)
+      else if (__any_sync(kFull, *static_cast<volatile int*>(&missed[cur]) != 0))
         take_back(row);
     } else if (warp == NW) {
       there = there && mbar_wait_bounded(&arrived[n & 3], phase, &gave_up, a.ctl.limit_ns);
@@ -863,9 +864,9 @@ distill_step_kernel(const Args<T> a)
 
 // ---------------------------------------------------------------------------------------
 // Gradients whose rows or lists do not fit the shared memory of a cluster (kGrad), and the loss alone: NT threads stream
-// their CTA's part of the row through shared memory (every thread its own vectors, kStreamDepth - 1 chunks of kStreamNv vectors under way),
-// and one more warp of rank 0's CTA takes the list. With kGrad every part is read a second time. Chunks are short so that
-// four CTAs fit an SM and one's beginning lies behind the others' chunks: 2048 x 131072 bf16 takes 113 us (4.8 TB/s),
+// their CTA's part of the row through shared memory (every thread its own vectors, kStreamDepth - 1 chunks of kStreamNv
+// vectors under way), and one more warp of rank 0's CTA takes the list. With kGrad every part is read a second time.
+// Chunks are short so that four CTAs fit an SM and one's beginning lies behind the others' chunks: 2048 x 131072 bf16 takes 113 us (4.8 TB/s),
 // 141 with chunks of eight vectors and two CTAs per SM, 130 with four vectors and a fourth stage.
 // ---------------------------------------------------------------------------------------
 constexpr int kStreamNv    = 4;
